@@ -265,6 +265,149 @@ jl_status jl_project_noalloc(jl_model* m, int layer, jl_projection which, const 
                              size_t rows, float* y, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Operators of tree-shaped speculation on device memory the caller owns.
+ * The reference drafts chains (speculative.rs:79-97) and grows its caches in
+ * place; these operators serve hosts that draft a tree of tokens, fork a
+ * sequence, or keep their own pages in the engine's layout.
+ *
+ * Conventions of this section
+ *  - Pointers are device pointers unless the text says otherwise, all on the
+ *    device that holds the pool; calls run there whichever device is current
+ *    (and leave the current device as it was).
+ *  - Calls are asynchronous on `stream`, a cudaStream_t (NULL: the device's
+ *    legacy default stream).  They allocate nothing, keep nothing from one
+ *    call for the next and can be captured into a CUDA graph.  Calls on
+ *    different streams are independent as long as their buffers are.
+ *  - A sequence's position p lies in page page_table[p / 64] of the pool, at
+ *    row p % 64.  Page ids outside [0, pages) and positions past the table
+ *    are never dereferenced: reads of them act as masked positions, writes
+ *    are skipped.
+ *  - `status` (nullable) points to a device int that the kernels OR bits
+ *    into: 1 a page id outside the pool, 2 an index or length out of range
+ *    (the part out of range was skipped), 4 a bounded device wait gave up
+ *    (the outputs of that call are not valid).
+ * ---------------------------------------------------------------------- */
+
+/* Pages of keys and values, [page][kv_head][64][128] of `dtype` for K and
+ * for V, 16-byte aligned.  Calls that work on every layer find layer l's
+ * pages layer_stride bytes times l behind k and v. */
+typedef struct jl_kv_pages {
+    void* k;
+    void* v;
+    size_t layer_stride;     /* a multiple of 16; ignored with one layer */
+    int layers;              /* 1 for the calls that work on one layer */
+    int pages;
+    int kv_heads;
+    jl_kv_dtype dtype;
+} jl_kv_pages;
+
+/* Per-head RMSNorm and rotation of queries and keys, and the append of keys
+ * and values to the cache, in one pass over the q|k|v rows of a projection
+ * (lib.rs:291-321, 363-396).  A row's rotation (pos) and its place in the
+ * sequence (slot) are separate: the nodes of a drafted tree at one depth
+ * share a position, and each has a slot of its own.
+ *   y = x / sqrt(mean(x^2) + eps) * w, then for i < 64
+ *   (y[i], y[i + 64]) -> (y[i] cos - y[i + 64] sin, y[i + 64] cos + y[i] sin)
+ * in f32, rounded once into q or the pool; values are stored as they come.
+ * A row whose pos lies outside [0, positions) is skipped whole (status 2).
+ * Two rows must not append to the same place. */
+typedef struct jl_norm_rope {
+    jl_kv_pages pool;          /* one layer */
+    int rows, q_heads;
+    jl_kv_dtype dtype;         /* type of the qkv and q rows */
+    const void* qkv;           /* [rows][qkv_ld]: q heads, k heads, v heads, 128 each; 16-byte aligned */
+    size_t qkv_ld;             /* elements from row to row, a multiple of 8 */
+    void* q;                   /* [rows][q_ld]: the rotated queries; may be qkv itself with q_ld == qkv_ld */
+    size_t q_ld;               /* a multiple of 8 */
+    const uint16_t* q_norm;    /* bf16 [128]; NULL: queries are rotated without a norm */
+    const uint16_t* k_norm;    /* bf16 [128]; NULL: keys are rotated without a norm */
+    float eps;
+    const float* rope;         /* [positions][64][2]: cos and sin of each angle */
+    int positions;
+    const int32_t* pos;        /* [rows] rotation position */
+    const int32_t* slot;       /* [rows] position in the sequence; negative: no append.  NULL: pos */
+    const int32_t* seq;        /* [rows] sequence (row of page_table).  NULL: sequence 0 */
+    const int32_t* page_table; /* [seqs][max_pages] */
+    int seqs, max_pages;
+    int32_t* status;
+} jl_norm_rope;
+jl_status jl_qk_norm_rope(const jl_norm_rope* a, void* stream);
+
+/* Most nodes a tree may have. */
+#define JL_TREE_MAX_NODES 256
+/* Workspace that is enough for every jl_tree_attention call. */
+#define JL_TREE_WORKSPACE_BYTES ((size_t)48 << 20)
+
+/* Attention of the nodes of drafted trees over the paged cache
+ * (lib.rs:401-441 for rows that do not form a chain).  Sequence s has the
+ * query rows row_start[s] .. row_start[s + 1] - 1, one per node, and ctx[s]
+ * committed positions that every node sees; node j's key and value lie at
+ * position ctx[s] + j and are seen by the nodes whose mask has bit j (a
+ * node's own bit included: nothing is added to the mask).  Without a mask
+ * the nodes form a chain: node i sees nodes 0..i, as in a prompt, a decode
+ * step or a linear verify pass.
+ *   out = sum over seen p of softmax(q . k_p * scale) v_p, in f32, rounded
+ *   once into the output type; lse = log of the sum of exp(q . k_p * scale).
+ * A row that sees nothing gets zeros and an lse of -infinity.  Whatever lies
+ * in positions that a row does not see, infinities and NaN included, does
+ * not reach its output.  Rows from row_start[seqs] on are not written.
+ * The sum is split between CTAs by the lengths of the whole batch, in a
+ * fixed order: the same inputs give the same bits, but a row's last bits may
+ * differ in another batch. */
+typedef struct jl_tree_attn {
+    jl_kv_pages pool;          /* one layer */
+    int rows, q_heads;         /* q_heads a multiple of pool.kv_heads, at most 128 per kv head */
+    jl_kv_dtype dtype;         /* type of the q and out rows */
+    const void* q;             /* [rows][q_ld], 16-byte aligned */
+    size_t q_ld;               /* elements from row to row, a multiple of 8 */
+    void* out;                 /* [rows][out_ld]; may be q itself with out_ld == q_ld */
+    size_t out_ld;             /* a multiple of 8 */
+    float* lse;                /* [rows][q_heads], or NULL */
+    int seqs;
+    int max_nodes;             /* largest tree of the batch, 1..JL_TREE_MAX_NODES */
+    const int32_t* row_start;  /* [seqs + 1] */
+    const int32_t* ctx;        /* [seqs] */
+    const uint64_t* mask;      /* [rows][mask_words]: bit j % 64 of word j / 64, or NULL */
+    int mask_words;            /* at least max_nodes / 64, rounded up */
+    const int32_t* page_table; /* [seqs][max_pages] */
+    int max_pages;
+    float scale;               /* 0: 1 / sqrt(128) */
+    void* workspace;           /* 256-byte aligned, not shared by calls that may overlap */
+    size_t workspace_bytes;    /* at least what jl_tree_attention_workspace says */
+    int32_t* status;
+} jl_tree_attn;
+jl_status jl_tree_attention(const jl_tree_attn* a, void* stream);
+/* Bytes of workspace the call needs (from its sizes alone; pointers may be
+ * NULL except pool.k, which names the device), at most
+ * JL_TREE_WORKSPACE_BYTES. */
+jl_status jl_tree_attention_workspace(const jl_tree_attn* a, size_t* bytes);
+
+/* Moves positions of sequences together in every layer: position ctx[s] + i
+ * takes what position ctx[s] + path[s][i] held before the call, for
+ * i < path_len[s] (the accepted path of a drafted tree; any order, entries
+ * may repeat).  Positions behind it keep what they held. */
+typedef struct jl_kv_compaction {
+    jl_kv_pages pool;
+    int seqs;
+    const int32_t* ctx;        /* [seqs] */
+    const int32_t* path;       /* [seqs][path_ld] node indices */
+    int path_ld;               /* 1..JL_TREE_MAX_NODES */
+    const int32_t* path_len;   /* [seqs], each at most path_ld */
+    const int32_t* page_table; /* [seqs][max_pages]; no page written by two sequences */
+    int max_pages;
+    int32_t* status;
+} jl_kv_compaction;
+jl_status jl_kv_compact(const jl_kv_compaction* a, void* stream);
+
+/* Copies n pages in every layer: the first rows[i] rows (1..64; rows NULL:
+ * all 64) of page src[i] to page dst[i], K and V.  src, dst and rows are
+ * host arrays, read before the call returns.  A page may be the source of
+ * several copies; a page that is the destination of two, or both source and
+ * destination, is an error. */
+jl_status jl_kv_copy_pages(const jl_kv_pages* pool, const int32_t* src, const int32_t* dst,
+                           const int32_t* rows, size_t n, void* stream);
+
+/* ------------------------------------------------------------------------
  * Profiling.
  * ---------------------------------------------------------------------- */
 

@@ -7,6 +7,7 @@
 #include <cstring>
 
 #include "jl_internal.h"
+#include "ops_host.h"
 
 namespace jl {
 
@@ -343,6 +344,34 @@ jl_status jl_time_projection(jl_model* m, int layer, jl_projection which, int ro
                              double* ms_per_launch, size_t* weight_bytes) {
     JL_NEED(m && ms_per_launch && weight_bytes, "model and outputs must be non-null");
     JL_GUARD({ return time_projection(m, layer, (int)which, rows, iters, ms_per_launch, weight_bytes); })
+}
+
+// ---- operators on device memory the caller owns -----------------------------------
+
+jl_status jl_qk_norm_rope(const jl_norm_rope* a, void* stream) {
+    JL_NEED(a, "arguments must be non-null");
+    JL_GUARD({ return qk_norm_rope(*a, (cudaStream_t)stream); })
+}
+
+jl_status jl_tree_attention(const jl_tree_attn* a, void* stream) {
+    JL_NEED(a, "arguments must be non-null");
+    JL_GUARD({ return tree::tree_attention(*a, (cudaStream_t)stream); })
+}
+
+jl_status jl_tree_attention_workspace(const jl_tree_attn* a, size_t* bytes) {
+    JL_NEED(a && bytes, "arguments and bytes must be non-null");
+    JL_GUARD({ return tree::tree_attention_workspace(*a, bytes); })
+}
+
+jl_status jl_kv_compact(const jl_kv_compaction* a, void* stream) {
+    JL_NEED(a, "arguments must be non-null");
+    JL_GUARD({ return kv_compact(*a, (cudaStream_t)stream); })
+}
+
+jl_status jl_kv_copy_pages(const jl_kv_pages* pool, const int32_t* src, const int32_t* dst, const int32_t* rows, size_t n,
+                           void* stream) {
+    JL_NEED(pool, "the pool must be non-null");
+    JL_GUARD({ return kv_copy_pages(*pool, src, dst, rows, n, (cudaStream_t)stream); })
 }
 
 jl_status jl_schedule_fixed(uint32_t gamma, jl_schedule* out) {

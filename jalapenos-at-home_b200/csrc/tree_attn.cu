@@ -1,0 +1,383 @@
+// Attention of the nodes of drafted trees over the paged cache
+// (jl_tree_attention): host checks, the CUDA-core kernel and the kernel that
+// adds the partial results of items that several workers share.
+#include <algorithm>
+#include <cmath>
+#include <mutex>
+
+#include "jl_internal.h"
+#include "launch.cuh"
+#include "ops_host.h"
+#include "ptx.cuh"
+#include "tree_attn.cuh"
+
+namespace jl {
+namespace tree {
+namespace {
+
+// 2^x, x <= 0 (ex2.approx.ftz: relative error about 2^-22).
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ float4 load4(const float* p) { return *(const float4*)p; }
+__device__ __forceinline__ float4 load4(const uint16_t* p) {
+    const uint2 w = *(const uint2*)p;
+    return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
+                       __uint_as_float(w.y & 0xffff0000u));
+}
+__device__ __forceinline__ void store4(float* p, float4 v) { *(float4*)p = v; }
+__device__ __forceinline__ void store4(uint16_t* p, float4 v) {
+    *(uint2*)p = make_uint2(f2bf16(v.x) | (uint32_t)f2bf16(v.y) << 16, f2bf16(v.z) | (uint32_t)f2bf16(v.w) << 16);
+}
+
+// ---- CUDA cores ------------------------------------------------------------------
+//
+// A CTA holds a tile of 16 * RT query rows and walks its range page by page:
+// K and V of a page go to shared memory as f32; thread (ty, tx) scores keys
+// tx + 16 i of rows ty + 16 j, the 16 threads of a row share its running
+// maximum and sum (online softmax, base 2), and each keeps dims 4 tx .. and
+// 64 + 4 tx .. of the row's output.
+constexpr int CC_T = 256;
+constexpr int CC_KLD = HEAD + 4;  // K rows padded: 8 rows' float4s on all banks
+constexpr int CC_PLD = PAGE + 4;
+
+template <int RT>
+constexpr size_t cc_smem() {
+    return sizeof(float) * ((size_t)16 * RT * CC_KLD + PAGE * CC_KLD + PAGE * HEAD + 16 * RT * CC_PLD);
+}
+
+template <typename KV, typename T, int RT>
+__global__ void __launch_bounds__(CC_T) k_tree_attn_cc(Args a) {
+    extern __shared__ __align__(16) float cc_smem_raw[];
+    float* qs = cc_smem_raw;                  // [16 RT][CC_KLD]
+    float* ks = qs + 16 * RT * CC_KLD;        // [PAGE][CC_KLD]
+    float* vs = ks + PAGE * CC_KLD;           // [PAGE][HEAD]
+    float* ps = vs + PAGE * HEAD;             // [16 RT][CC_PLD]
+    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+    const int worker = blockIdx.x, lane = blockIdx.y;
+    constexpr int R = 16 * RT;
+    ptx::grid_dependency_wait();
+    ptx::launch_dependents();
+    int s;
+    long long first;
+    const Split sp = locate<CC_T>(a, worker, &s, &first);
+    Walk w;
+    if (worker >= sp.used || !w.start(a, s, first, sp.at(worker), sp.at(worker + 1))) return;
+    do {
+        const int live = min(R, w.q.n * a.group - lane * R);  // rows of this tile
+        if (live <= 0) continue;
+        __syncthreads();  // the previous segment's tiles are no longer read
+        for (int i = tid; i < R * 32; i += CC_T) {
+            const int r = i >> 5, c = i & 31, g = lane * R + r;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < live)
+                v = load4((const T*)a.q + (size_t)(w.q.lo + g / a.group) * a.q_ld +
+                          (size_t)(w.h * a.group + g % a.group) * HEAD + 4 * c);
+            *(float4*)(qs + r * CC_KLD + 4 * c) = v;
+        }
+        float m[RT], l[RT], acc[RT][8];
+#pragma unroll
+        for (int j = 0; j < RT; ++j) {
+            m[j] = -INFINITY;
+            l[j] = 0.f;
+#pragma unroll
+            for (int d = 0; d < 8; ++d) acc[j][d] = 0.f;
+        }
+        const int32_t* pt = a.page_table + (size_t)w.s * a.max_pages;
+        for (int p = w.p0; p < w.p1; ++p) {
+            const int page = pt[p];
+            const bool there = (unsigned)page < (unsigned)a.pages;
+            if (!there && tid == 0) flag(a.status, ST_PAGE);
+            const int used = there ? (int)min((long long)PAGE, (long long)w.q.ctx + w.q.n - (long long)p * PAGE) : 0;
+            __syncthreads();  // the previous page's tiles are no longer read
+            const size_t at = kv_index(there ? page : 0, w.h, 0, a.kv_heads);
+            for (int i = tid; i < PAGE * 32; i += CC_T) {
+                const int r = i >> 5, c = i & 31;
+                float4 kk = make_float4(0.f, 0.f, 0.f, 0.f), vv = kk;
+                if (r < used) {  // rows past the sequence may hold anything
+                    kk = load4((const KV*)a.k + at + (size_t)r * HEAD + 4 * c);
+                    vv = load4((const KV*)a.v + at + (size_t)r * HEAD + 4 * c);
+                }
+                *(float4*)(ks + r * CC_KLD + 4 * c) = kk;
+                *(float4*)(vs + r * HEAD + 4 * c) = vv;
+            }
+            __syncthreads();
+            const bool edge = (long long)(p + 1) * PAGE > w.q.ctx || !there;
+            uint64_t vis[RT];
+#pragma unroll
+            for (int j = 0; j < RT; ++j) {
+                const int r = ty + 16 * j;
+                vis[j] = !there || r >= live ? 0 : edge ? visible(a, w.q, (lane * R + r) / a.group, p) : ~0ull;
+                float sc[4] = {0.f, 0.f, 0.f, 0.f};
+                const float* qr = qs + r * CC_KLD;
+#pragma unroll 8
+                for (int c = 0; c < 32; ++c) {
+                    const float4 q4 = *(const float4*)(qr + 4 * c);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float4 k4 = *(const float4*)(ks + (tx + 16 * i) * CC_KLD + 4 * c);
+                        sc[i] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, sc[i]))));
+                    }
+                }
+                float top = m[j];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    sc[i] = vis[j] >> (tx + 16 * i) & 1 ? __fmul_rn(sc[i], a.c2) : -INFINITY;
+                    top = fmaxf(top, sc[i]);
+                }
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                const float ref = top == -INFINITY ? 0.f : top;
+                const float corr = ex2(m[j] - ref);  // 0 while nothing was seen
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float e = vis[j] >> (tx + 16 * i) & 1 ? ex2(sc[i] - ref) : 0.f;
+                    ps[r * CC_PLD + tx + 16 * i] = e;
+                    sum += e;
+                }
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                l[j] = fmaf(l[j], corr, sum);
+                m[j] = top;
+#pragma unroll
+                for (int d = 0; d < 8; ++d) acc[j][d] *= corr;
+            }
+            __syncwarp();  // a row's weights are read by the half warp that wrote them
+            for (int key = 0; key < PAGE; ++key) {
+                const float4 v0 = *(const float4*)(vs + key * HEAD + 4 * tx);
+                const float4 v1 = *(const float4*)(vs + key * HEAD + 64 + 4 * tx);
+#pragma unroll
+                for (int j = 0; j < RT; ++j) {
+                    // not seen: skipped, not multiplied by zero (V may be infinite)
+                    if (edge && !(vis[j] >> key & 1)) continue;
+                    const float e = ps[(ty + 16 * j) * CC_PLD + key];
+                    acc[j][0] = fmaf(e, v0.x, acc[j][0]);
+                    acc[j][1] = fmaf(e, v0.y, acc[j][1]);
+                    acc[j][2] = fmaf(e, v0.z, acc[j][2]);
+                    acc[j][3] = fmaf(e, v0.w, acc[j][3]);
+                    acc[j][4] = fmaf(e, v1.x, acc[j][4]);
+                    acc[j][5] = fmaf(e, v1.y, acc[j][5]);
+                    acc[j][6] = fmaf(e, v1.z, acc[j][6]);
+                    acc[j][7] = fmaf(e, v1.w, acc[j][7]);
+                }
+            }
+        }
+        const bool whole = w.whole();
+        const size_t part = (((size_t)worker * a.lanes + lane) * 2 + w.slot()) * R;
+#pragma unroll
+        for (int j = 0; j < RT; ++j) {
+            const int r = ty + 16 * j, g = lane * R + r;
+            if (r >= live) continue;
+            float4 o0 = make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
+            float4 o1 = make_float4(acc[j][4], acc[j][5], acc[j][6], acc[j][7]);
+            if (whole) {
+                const float inv = m[j] == -INFINITY ? 0.f : __fdiv_rn(1.f, l[j]);
+                const int row = w.q.lo + g / a.group, head = w.h * a.group + g % a.group;
+                T* dst = (T*)a.out + (size_t)row * a.out_ld + (size_t)head * HEAD;
+                store4(dst + 4 * tx, make_float4(o0.x * inv, o0.y * inv, o0.z * inv, o0.w * inv));
+                store4(dst + 64 + 4 * tx, make_float4(o1.x * inv, o1.y * inv, o1.z * inv, o1.w * inv));
+                if (a.lse && tx == 0)
+                    a.lse[(size_t)row * a.q_heads + head] =
+                        m[j] == -INFINITY ? -INFINITY : (m[j] + log2f(l[j])) * 0.6931471805599453f;
+            } else {
+                store4(a.ws_o + (part + r) * HEAD + 4 * tx, o0);
+                store4(a.ws_o + (part + r) * HEAD + 64 + 4 * tx, o1);
+                if (tx == 0) *(float2*)(a.ws_ml + (part + r) * 2) = make_float2(m[j], l[j]);
+            }
+        }
+    } while (w.next(a));
+}
+
+// ---- partial results -----------------------------------------------------------------
+//
+// Block (w, lane, z): if worker w's range starts inside an item and is the
+// first to do so, the item's partials, from worker w - 1 on, are added in
+// order: a warp per row, lane l holding dims 4 l ...  z deals the rows out.
+constexpr int CB_T = 256;
+
+template <typename T>
+__global__ void __launch_bounds__(CB_T) k_tree_combine(Args a) {
+    const int w = blockIdx.x + 1, lane = blockIdx.y;
+    const int warp = threadIdx.x >> 5, l = threadIdx.x & 31;
+    ptx::grid_dependency_wait();
+    ptx::launch_dependents();
+    int s;
+    long long first;
+    const Split sp = locate<CB_T>(a, w, &s, &first);
+    if (w >= sp.used || s >= a.seqs) return;
+    const Seq q = seq_of(a, s);
+    const long long u = sp.at(w);
+    const int h = (int)((u - first) / q.np);
+    const long long item = first + (long long)h * q.np, item_end = item + q.np;
+    if (u == item || sp.at(w - 1) > item) return;  // starts on an item, or not the first inside it
+    int last = w;
+    while (sp.at(last + 1) < item_end) ++last;
+    const int R = a.tile_rows, live = min(R, q.n * a.group - lane * R);
+    for (int r = blockIdx.z * (CB_T / 32) + warp; r < live; r += gridDim.z * (CB_T / 32)) {
+        // worker w - 1 began the item unless its range starts exactly on it, or
+        // before it: its partial is then the one of the item its range ends in
+        auto slot = [&](int x) { return (((size_t)x * a.lanes + lane) * 2 + (x == w - 1 ? 1 : 0)) * R + r; };
+        float top = -INFINITY;
+        for (int x = w - 1 + l; x <= last; x += 32) top = fmaxf(top, a.ws_ml[slot(x) * 2]);
+        top = warp_max(top);
+        const float ref = top == -INFINITY ? 0.f : top;
+        float sum = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int x = w - 1; x <= last; ++x) {
+            const float2 ml = *(const float2*)(a.ws_ml + slot(x) * 2);
+            const float4 v = *(const float4*)(a.ws_o + slot(x) * HEAD + 4 * l);
+            if (ml.x == -INFINITY) continue;
+            const float f = ex2(ml.x - ref);
+            sum = fmaf(ml.y, f, sum);
+            o.x = fmaf(v.x, f, o.x);
+            o.y = fmaf(v.y, f, o.y);
+            o.z = fmaf(v.z, f, o.z);
+            o.w = fmaf(v.w, f, o.w);
+        }
+        const float inv = top == -INFINITY ? 0.f : __fdiv_rn(1.f, sum);
+        const int g = lane * R + r, row = q.lo + g / a.group, head = h * a.group + g % a.group;
+        store4((T*)a.out + (size_t)row * a.out_ld + (size_t)head * HEAD + 4 * l,
+               make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+        if (a.lse && l == 0)
+            a.lse[(size_t)row * a.q_heads + head] =
+                top == -INFINITY ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+    }
+}
+
+// ---- host ----------------------------------------------------------------------------
+
+// The kernel that a call takes and how it cuts the work.
+struct Plan {
+    int tile_rows, lanes, workers, min_units;
+    size_t bytes;
+};
+
+Plan plan_of(const jl_tree_attn& a, int sms) {
+    Plan p;
+    const int rows = a.max_nodes * (a.q_heads / a.pool.kv_heads);
+    p.tile_rows = rows <= 16 ? 16 : 64;
+    p.lanes = (rows + p.tile_rows - 1) / p.tile_rows;
+    p.workers = std::max(1, sms / p.lanes);
+    p.min_units = 2;
+    p.bytes = p.workers == 1 ? 0 : (size_t)p.workers * p.lanes * 2 * p.tile_rows * (HEAD + 2) * sizeof(float);
+    return p;
+}
+
+template <typename KV, typename T>
+jl_status launch_cc(const Args& a, cudaStream_t st) {
+    const dim3 grid(a.workers, a.lanes);
+    if (a.tile_rows == 16) return launch_pdl(k_tree_attn_cc<KV, T, 1>, grid, dim3(CC_T), cc_smem<1>(), st, a);
+    return launch_pdl(k_tree_attn_cc<KV, T, 4>, grid, dim3(CC_T), cc_smem<4>(), st, a);
+}
+
+template <typename KV, typename T>
+jl_status configure_cc() {
+    JL_CUDA(cudaFuncSetAttribute(k_tree_attn_cc<KV, T, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cc_smem<1>()));
+    JL_CUDA(cudaFuncSetAttribute(k_tree_attn_cc<KV, T, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cc_smem<4>()));
+    return JL_OK;
+}
+
+jl_status configure(int device) {  // once per device
+    static std::mutex mu;
+    static bool done[64] = {};
+    std::lock_guard<std::mutex> g(mu);
+    if (device < 64 && done[device]) return JL_OK;
+    JL_TRY((configure_cc<float, float>()));
+    JL_TRY((configure_cc<float, uint16_t>()));
+    JL_TRY((configure_cc<uint16_t, float>()));
+    JL_TRY((configure_cc<uint16_t, uint16_t>()));
+    if (device < 64) done[device] = true;
+    return JL_OK;
+}
+
+jl_status check_sizes(const jl_tree_attn& a) {
+    JL_REFUSE(a.rows < 0 || a.seqs < 0, "tree attention: rows and seqs must not be negative");
+    JL_TRY(check_pages(a.pool, true));
+    JL_REFUSE(a.q_heads < 1 || a.q_heads % a.pool.kv_heads || a.q_heads / a.pool.kv_heads > 128,
+              "tree attention: %d query heads over %d kv heads (a multiple, at most 128 per kv head)", a.q_heads,
+              a.pool.kv_heads);
+    JL_REFUSE(a.max_nodes < 1 || a.max_nodes > JL_TREE_MAX_NODES, "tree attention: max_nodes must be 1..%d, got %d",
+              JL_TREE_MAX_NODES, a.max_nodes);
+    JL_REFUSE(a.dtype != JL_KV_BF16 && a.dtype != JL_KV_F32, "tree attention: dtype must be bf16 or f32");
+    return JL_OK;
+}
+
+}  // namespace
+
+jl_status tree_attention(const jl_tree_attn& a, cudaStream_t st) {
+    JL_TRY(check_sizes(a));
+    JL_REFUSE(!a.q || !a.out || !a.row_start || !a.ctx || !a.page_table,
+              "tree attention: q, out, row_start, ctx and page_table must be non-null");
+    const size_t width = (size_t)a.q_heads * HEAD;
+    JL_REFUSE(a.q_ld < width || a.out_ld < width || a.q_ld % 8 || a.out_ld % 8,
+              "tree attention: q_ld and out_ld must be multiples of 8 and at least %zu", width);
+    JL_REFUSE(misaligned(a.q) || misaligned(a.out), "tree attention: q and out must be 16-byte aligned");
+    JL_REFUSE(a.q == a.out && a.q_ld != a.out_ld, "tree attention: out over q needs out_ld == q_ld");
+    JL_REFUSE(a.mask && (long long)a.mask_words * 64 < a.max_nodes, "tree attention: %d mask words hold fewer than %d nodes",
+              a.mask_words, a.max_nodes);
+    JL_REFUSE(a.max_pages < 1 || a.max_pages > MAX_TABLE, "tree attention: max_pages must be 1..%d", MAX_TABLE);
+    JL_REFUSE(!(a.scale >= 0.f) || std::isinf(a.scale), "tree attention: scale must be finite and not negative");
+    if (a.rows == 0 || a.seqs == 0) return JL_OK;
+    DeviceOf on;
+    JL_TRY(on.enter(a.pool.k, "tree attention: pool.k"));
+    JL_TRY(configure(on.device));
+    const Plan p = plan_of(a, on.sms);
+    JL_REFUSE(p.bytes && (!a.workspace || ((uintptr_t)a.workspace & 255)),
+              "tree attention: the workspace must be 256-byte aligned device memory");
+    JL_REFUSE(a.workspace_bytes < p.bytes, "tree attention: workspace of %zu bytes, %zu needed", a.workspace_bytes, p.bytes);
+    Args k{};
+    k.q = a.q;
+    k.out = a.out;
+    k.lse = a.lse;
+    k.q_ld = (long long)a.q_ld;
+    k.out_ld = (long long)a.out_ld;
+    k.rows = a.rows;
+    k.q_heads = a.q_heads;
+    k.kv_heads = a.pool.kv_heads;
+    k.group = a.q_heads / a.pool.kv_heads;
+    k.seqs = a.seqs;
+    k.max_nodes = a.max_nodes;
+    k.row_start = a.row_start;
+    k.ctx = a.ctx;
+    k.mask = a.mask;
+    k.mask_words = a.mask_words;
+    k.page_table = a.page_table;
+    k.max_pages = a.max_pages;
+    k.pages = a.pool.pages;
+    k.k = a.pool.k;
+    k.v = a.pool.v;
+    k.c2 = (float)((a.scale == 0.f ? 1.0 / std::sqrt((double)HEAD) : (double)a.scale) * 1.4426950408889634);
+    k.workers = p.workers;
+    k.lanes = p.lanes;
+    k.tile_rows = p.tile_rows;
+    k.min_units = p.min_units;
+    k.ws_o = (float*)a.workspace;
+    k.ws_ml = k.ws_o + (size_t)p.workers * p.lanes * 2 * p.tile_rows * HEAD;
+    k.status = a.status;
+    const bool f = a.dtype == JL_KV_F32;
+    if (a.pool.dtype == JL_KV_F32) JL_TRY((f ? launch_cc<float, float>(k, st) : launch_cc<float, uint16_t>(k, st)));
+    else JL_TRY((f ? launch_cc<uint16_t, float>(k, st) : launch_cc<uint16_t, uint16_t>(k, st)));
+    if (p.workers > 1) {
+        // enough blocks that a tile's rows are added at once
+        const dim3 grid(p.workers - 1, p.lanes, std::max(1, p.tile_rows / (CB_T / 32)));
+        JL_TRY((f ? launch_pdl(k_tree_combine<float>, grid, dim3(CB_T), 0, st, k)
+                  : launch_pdl(k_tree_combine<uint16_t>, grid, dim3(CB_T), 0, st, k)));
+    }
+    return JL_OK;
+}
+
+jl_status tree_attention_workspace(const jl_tree_attn& a, size_t* bytes) {
+    JL_TRY(check_sizes(a));
+    DeviceOf on;
+    JL_TRY(on.enter(a.pool.k, "tree attention: pool.k"));
+    *bytes = plan_of(a, on.sms).bytes;
+    return JL_OK;
+}
+
+}  // namespace tree
+}  // namespace jl

@@ -40,7 +40,8 @@ EXPORTS = (
     "jl_generate_speculative", "jl_time_pass", "jl_time_projection", "jl_project",
     "jl_project_noalloc", "jl_pass_kernels", "jl_time_pass_draft", "jl_generate_batch",
     "jl_generate_speculative_batch", "jl_timeline_read", "jl_timeline_kernel", "jl_wait_probe",
-    "jl_model_prompt_attention",
+    "jl_model_prompt_attention", "jl_qk_norm_rope", "jl_tree_attention", "jl_tree_attention_workspace",
+    "jl_kv_compact", "jl_kv_copy_pages",
 )
 PROJ_QKV, PROJ_O, PROJ_GATE_UP, PROJ_DOWN, PROJ_HEAD = 0, 1, 2, 3, 4
 
@@ -110,6 +111,37 @@ class BatchStats(ctypes.Structure):
                 ("target_passes", ctypes.c_size_t), ("draft_passes", ctypes.c_size_t)]
 
 
+class KvPages(ctypes.Structure):
+    """Pages of keys and values in device memory (see jl_kv_pages)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("layer_stride", ctypes.c_size_t),
+                ("layers", ctypes.c_int), ("pages", ctypes.c_int), ("kv_heads", ctypes.c_int), ("dtype", ctypes.c_int)]
+
+
+class NormRope(ctypes.Structure):
+    _fields_ = [("pool", KvPages), ("rows", ctypes.c_int), ("q_heads", ctypes.c_int), ("dtype", ctypes.c_int),
+                ("qkv", ctypes.c_void_p), ("qkv_ld", ctypes.c_size_t), ("q", ctypes.c_void_p), ("q_ld", ctypes.c_size_t),
+                ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p), ("eps", ctypes.c_float),
+                ("rope", ctypes.c_void_p), ("positions", ctypes.c_int), ("pos", ctypes.c_void_p),
+                ("slot", ctypes.c_void_p), ("seq", ctypes.c_void_p), ("page_table", ctypes.c_void_p),
+                ("seqs", ctypes.c_int), ("max_pages", ctypes.c_int), ("status", ctypes.c_void_p)]
+
+
+class TreeAttn(ctypes.Structure):
+    _fields_ = [("pool", KvPages), ("rows", ctypes.c_int), ("q_heads", ctypes.c_int), ("dtype", ctypes.c_int),
+                ("q", ctypes.c_void_p), ("q_ld", ctypes.c_size_t), ("out", ctypes.c_void_p), ("out_ld", ctypes.c_size_t),
+                ("lse", ctypes.c_void_p), ("seqs", ctypes.c_int), ("max_nodes", ctypes.c_int),
+                ("row_start", ctypes.c_void_p), ("ctx", ctypes.c_void_p), ("mask", ctypes.c_void_p),
+                ("mask_words", ctypes.c_int), ("page_table", ctypes.c_void_p), ("max_pages", ctypes.c_int),
+                ("scale", ctypes.c_float), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+                ("status", ctypes.c_void_p)]
+
+
+class KvCompaction(ctypes.Structure):
+    _fields_ = [("pool", KvPages), ("seqs", ctypes.c_int), ("ctx", ctypes.c_void_p), ("path", ctypes.c_void_p),
+                ("path_ld", ctypes.c_int), ("path_len", ctypes.c_void_p), ("page_table", ctypes.c_void_p),
+                ("max_pages", ctypes.c_int), ("status", ctypes.c_void_p)]
+
+
 def _load():
     if not LIB_PATH.exists():
         raise ImportError(f"{LIB_PATH} is missing: build it with `make -C {HERE}` "
@@ -165,6 +197,12 @@ def _load():
         "jl_timeline_kernel": ([sz], ctypes.c_char_p),
         "jl_wait_probe": ([vp, ctypes.c_uint32], ctypes.c_int),
         "jl_model_prompt_attention": ([vp, ctypes.c_int, ctypes.POINTER(ctypes.c_int)], ctypes.c_int),
+        "jl_qk_norm_rope": ([ctypes.POINTER(NormRope), vp], ctypes.c_int),
+        "jl_tree_attention": ([ctypes.POINTER(TreeAttn), vp], ctypes.c_int),
+        "jl_tree_attention_workspace": ([ctypes.POINTER(TreeAttn), ctypes.POINTER(sz)], ctypes.c_int),
+        "jl_kv_compact": ([ctypes.POINTER(KvCompaction), vp], ctypes.c_int),
+        "jl_kv_copy_pages": ([ctypes.POINTER(KvPages), ctypes.POINTER(ctypes.c_int32),
+                              ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int32), sz, vp], ctypes.c_int),
     }
     for name, (args, res) in sig.items():
         fn = getattr(L, name)
@@ -625,6 +663,70 @@ def generate_speculative_batch(target: Model, draft: Model, prompts, count: int,
     check(lib.jl_generate_speculative_batch(target._h, draft._h, B, ptrs, lens, count, sc, opts, res,
                                             ctypes.byref(stats)))
     return _batch_result(outs, rounds, res, stats)
+
+
+# ---------------------------------------------------------------------------
+# operators of tree-shaped speculation on device memory the caller owns.
+# Arguments are device addresses (ints) and sizes; every call is asynchronous
+# on `stream`, a cudaStream_t handle (0: the device's legacy default stream).
+# The structures of the same names in include/jalapeno.h say what each holds.
+
+TREE_MAX_NODES = 256
+TREE_WORKSPACE_BYTES = 48 << 20
+
+
+def kv_pages(k: int, v: int, pages: int, kv_heads: int, dtype: int = KV_BF16, layers: int = 1,
+             layer_stride: int = 0) -> KvPages:
+    """Pages of keys and values at device addresses ``k`` and ``v``, each
+    [page][kv_head][64][128]; layer l lies l * layer_stride bytes behind."""
+    return KvPages(k, v, layer_stride, layers, pages, kv_heads, dtype)
+
+
+def qk_norm_rope(pool: KvPages, *, qkv: int, qkv_ld: int, q: int, q_ld: int, rows: int, q_heads: int, rope: int,
+                 positions: int, pos: int, page_table: int, max_pages: int, dtype: int = KV_F32, q_norm: int = 0,
+                 k_norm: int = 0, eps: float = 1e-6, slot: int = 0, seq: int = 0, seqs: int = 1, status: int = 0,
+                 stream: int = 0) -> None:
+    """Per-head norms and rotation of the q and k heads of q|k|v rows, and the
+    append of keys and values to the pages (jl_qk_norm_rope)."""
+    a = NormRope(pool, rows, q_heads, dtype, qkv, qkv_ld, q, q_ld, q_norm, k_norm, eps, rope, positions, pos, slot,
+                 seq, page_table, seqs, max_pages, status)
+    check(lib.jl_qk_norm_rope(a, stream))
+
+
+def tree_attention(pool: KvPages, *, q: int, q_ld: int, out: int, out_ld: int, rows: int, q_heads: int, seqs: int,
+                   max_nodes: int, row_start: int, ctx: int, page_table: int, max_pages: int, workspace: int,
+                   workspace_bytes: int, mask: int = 0, mask_words: int = 0, dtype: int = KV_F32, scale: float = 0.0,
+                   lse: int = 0, status: int = 0, stream: int = 0) -> None:
+    """Attention of the nodes of drafted trees over the paged cache
+    (jl_tree_attention)."""
+    a = TreeAttn(pool, rows, q_heads, dtype, q, q_ld, out, out_ld, lse, seqs, max_nodes, row_start, ctx, mask,
+                 mask_words, page_table, max_pages, scale, workspace, workspace_bytes, status)
+    check(lib.jl_tree_attention(a, stream))
+
+
+def tree_attention_workspace(pool: KvPages, *, q_heads: int, max_nodes: int, dtype: int = KV_F32) -> int:
+    """Bytes of workspace a tree_attention call of these sizes needs."""
+    a = TreeAttn(pool=pool, q_heads=q_heads, dtype=dtype, max_nodes=max_nodes)
+    n = ctypes.c_size_t()
+    check(lib.jl_tree_attention_workspace(a, ctypes.byref(n)))
+    return n.value
+
+
+def kv_compact(pool: KvPages, *, seqs: int, ctx: int, path: int, path_ld: int, path_len: int, page_table: int,
+               max_pages: int, status: int = 0, stream: int = 0) -> None:
+    """Moves accepted nodes' rows together in every layer (jl_kv_compact)."""
+    a = KvCompaction(pool, seqs, ctx, path, path_ld, path_len, page_table, max_pages, status)
+    check(lib.jl_kv_compact(a, stream))
+
+
+def kv_copy_pages(pool: KvPages, src, dst, rows=None, stream: int = 0) -> None:
+    """Copies pages src[i] to dst[i] in every layer, the first rows[i] rows of
+    each (jl_kv_copy_pages); src, dst and rows are host sequences."""
+    n = len(src)
+    if len(dst) != n or (rows is not None and len(rows) != n):
+        raise ValueError("src, dst and rows must have the same length")
+    ints = ctypes.c_int32 * n
+    check(lib.jl_kv_copy_pages(pool, ints(*src), ints(*dst), None if rows is None else ints(*rows), n, stream))
 
 
 def _philox4x32_10(c0, c1, c2, c3, k0: int, k1: int):
