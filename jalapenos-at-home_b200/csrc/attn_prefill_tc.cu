@@ -459,35 +459,39 @@ bool prefill_tc_supported(const jl_model* m) {
     return group == 1 || group == 2 || group == 4 || group == 8;
 }
 
-// Two tensor maps per layer over its K and V pages: rows (page, kv head,
-// slot) of HEAD bf16, boxes of 64 dims x one page, 128-byte swizzle.
-jl_status kv_tensor_maps(jl_model* m) {
-    m->kv_tmaps.clear();
-    if (m->kv.dtype != JL_KV_BF16) return JL_OK;
-    const uint64_t rows = (uint64_t)m->kv.pages * m->kv_heads * PAGE;
-    if (rows >= (1ull << 31)) return JL_OK;  // row coordinates are 32-bit
+// The TMA view of one layer's K or V pages: rows (page, kv head, slot) of HEAD
+// bf16, boxes of 64 dims x one page, 128-byte swizzle.
+jl_status kv_page_map(CUtensorMap* map, void* pages, uint64_t rows) {
     PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
     if (!enc) {
         set_error("cuTensorMapEncodeTiled is not available from the driver");
         return JL_ERR_CUDA;
     }
+    const cuuint64_t dims[2] = {(cuuint64_t)HEAD, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)HEAD * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)PAGE};
+    const cuuint32_t es[2] = {1, 1};
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, pages, dims, strides, box, es,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_error("cuTensorMapEncodeTiled failed (%d) for KV pages at %p", (int)r, pages);
+        return JL_ERR_CUDA;
+    }
+    return JL_OK;
+}
+
+// Two tensor maps per layer over its K and V pages.
+jl_status kv_tensor_maps(jl_model* m) {
+    m->kv_tmaps.clear();
+    if (m->kv.dtype != JL_KV_BF16) return JL_OK;
+    const uint64_t rows = (uint64_t)m->kv.pages * m->kv_heads * PAGE;
+    if (rows >= (1ull << 31)) return JL_OK;  // row coordinates are 32-bit
     std::vector<CUtensorMap> maps((size_t)2 * m->layers);
     for (int l = 0; l < m->layers; ++l) {
         const KvView v = kv_view(m, l);
-        for (int which = 0; which < 2; ++which) {
-            const cuuint64_t dims[2] = {(cuuint64_t)HEAD, (cuuint64_t)rows};
-            const cuuint64_t strides[1] = {(cuuint64_t)HEAD * 2};
-            const cuuint32_t box[2] = {64, (cuuint32_t)PAGE};
-            const cuuint32_t es[2] = {1, 1};
-            const CUresult r = enc(&maps[(size_t)2 * l + which], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
-                                   which ? v.v : v.k, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-            if (r != CUDA_SUCCESS) {
-                set_error("cuTensorMapEncodeTiled failed (%d) for the KV pages of layer %d", (int)r, l);
-                return JL_ERR_CUDA;
-            }
-        }
+        JL_TRY(kv_page_map(&maps[(size_t)2 * l], v.k, rows));
+        JL_TRY(kv_page_map(&maps[(size_t)2 * l + 1], v.v, rows));
     }
     m->kv_tmaps.swap(maps);
     return JL_OK;

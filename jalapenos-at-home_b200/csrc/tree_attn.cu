@@ -15,13 +15,6 @@ namespace jl {
 namespace tree {
 namespace {
 
-// 2^x, x <= 0 (ex2.approx.ftz: relative error about 2^-22).
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 __device__ __forceinline__ float4 load4(const float* p) { return *(const float4*)p; }
 __device__ __forceinline__ float4 load4(const uint16_t* p) {
     const uint2 w = *(const uint2*)p;
@@ -33,7 +26,7 @@ __device__ __forceinline__ void store4(uint16_t* p, float4 v) {
     *(uint2*)p = make_uint2(f2bf16(v.x) | (uint32_t)f2bf16(v.y) << 16, f2bf16(v.z) | (uint32_t)f2bf16(v.w) << 16);
 }
 
-// ---- CUDA cores ------------------------------------------------------------------
+// ---- CUDA cores: pools of f32 pages -----------------------------------------------
 //
 // A CTA holds a tile of 16 * RT query rows and walks its range page by page:
 // K and V of a page go to shared memory as f32; thread (ty, tx) scores keys
@@ -49,7 +42,7 @@ constexpr size_t cc_smem() {
     return sizeof(float) * ((size_t)16 * RT * CC_KLD + PAGE * CC_KLD + PAGE * HEAD + 16 * RT * CC_PLD);
 }
 
-template <typename KV, typename T, int RT>
+template <typename T, int RT>
 __global__ void __launch_bounds__(CC_T) k_tree_attn_cc(Args a) {
     extern __shared__ __align__(16) float cc_smem_raw[];
     float* qs = cc_smem_raw;                  // [16 RT][CC_KLD]
@@ -61,9 +54,10 @@ __global__ void __launch_bounds__(CC_T) k_tree_attn_cc(Args a) {
     constexpr int R = 16 * RT;
     ptx::grid_dependency_wait();
     ptx::launch_dependents();
+    __shared__ LocateScratch scratch;
     int s;
     long long first;
-    const Split sp = locate<CC_T>(a, worker, &s, &first);
+    const Split sp = locate<CC_T>(a, worker, scratch, &s, &first);
     Walk w;
     if (worker >= sp.used || !w.start(a, s, first, sp.at(worker), sp.at(worker + 1))) return;
     do {
@@ -98,8 +92,8 @@ __global__ void __launch_bounds__(CC_T) k_tree_attn_cc(Args a) {
                 const int r = i >> 5, c = i & 31;
                 float4 kk = make_float4(0.f, 0.f, 0.f, 0.f), vv = kk;
                 if (r < used) {  // rows past the sequence may hold anything
-                    kk = load4((const KV*)a.k + at + (size_t)r * HEAD + 4 * c);
-                    vv = load4((const KV*)a.v + at + (size_t)r * HEAD + 4 * c);
+                    kk = load4((const float*)a.k + at + (size_t)r * HEAD + 4 * c);
+                    vv = load4((const float*)a.v + at + (size_t)r * HEAD + 4 * c);
                 }
                 *(float4*)(ks + r * CC_KLD + 4 * c) = kk;
                 *(float4*)(vs + r * HEAD + 4 * c) = vv;
@@ -175,14 +169,14 @@ __global__ void __launch_bounds__(CC_T) k_tree_attn_cc(Args a) {
             float4 o0 = make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
             float4 o1 = make_float4(acc[j][4], acc[j][5], acc[j][6], acc[j][7]);
             if (whole) {
-                const float inv = m[j] == -INFINITY ? 0.f : __fdiv_rn(1.f, l[j]);
+                const float inv = l[j] == 0.f ? 0.f : __fdiv_rn(1.f, l[j]);  // 0: nothing seen
                 const int row = w.q.lo + g / a.group, head = w.h * a.group + g % a.group;
                 T* dst = (T*)a.out + (size_t)row * a.out_ld + (size_t)head * HEAD;
                 store4(dst + 4 * tx, make_float4(o0.x * inv, o0.y * inv, o0.z * inv, o0.w * inv));
                 store4(dst + 64 + 4 * tx, make_float4(o1.x * inv, o1.y * inv, o1.z * inv, o1.w * inv));
                 if (a.lse && tx == 0)
                     a.lse[(size_t)row * a.q_heads + head] =
-                        m[j] == -INFINITY ? -INFINITY : (m[j] + log2f(l[j])) * 0.6931471805599453f;
+                        l[j] == 0.f ? -INFINITY : (m[j] + log2f(l[j])) * LN2;
             } else {
                 store4(a.ws_o + (part + r) * HEAD + 4 * tx, o0);
                 store4(a.ws_o + (part + r) * HEAD + 64 + 4 * tx, o1);
@@ -205,9 +199,10 @@ __global__ void __launch_bounds__(CB_T) k_tree_combine(Args a) {
     const int warp = threadIdx.x >> 5, l = threadIdx.x & 31;
     ptx::grid_dependency_wait();
     ptx::launch_dependents();
+    __shared__ LocateScratch scratch;
     int s;
     long long first;
-    const Split sp = locate<CB_T>(a, w, &s, &first);
+    const Split sp = locate<CB_T>(a, w, scratch, &s, &first);
     if (w >= sp.used || s >= a.seqs) return;
     const Seq q = seq_of(a, s);
     const long long u = sp.at(w);
@@ -231,21 +226,20 @@ __global__ void __launch_bounds__(CB_T) k_tree_combine(Args a) {
         for (int x = w - 1; x <= last; ++x) {
             const float2 ml = *(const float2*)(a.ws_ml + slot(x) * 2);
             const float4 v = *(const float4*)(a.ws_o + slot(x) * HEAD + 4 * l);
-            if (ml.x == -INFINITY) continue;
-            const float f = ex2(ml.x - ref);
+            const float f = ml.y == 0.f ? 0.f : ex2(ml.x - ref);  // 0: nothing seen there
             sum = fmaf(ml.y, f, sum);
             o.x = fmaf(v.x, f, o.x);
             o.y = fmaf(v.y, f, o.y);
             o.z = fmaf(v.z, f, o.z);
             o.w = fmaf(v.w, f, o.w);
         }
-        const float inv = top == -INFINITY ? 0.f : __fdiv_rn(1.f, sum);
+        const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
         const int g = lane * R + r, row = q.lo + g / a.group, head = h * a.group + g % a.group;
         store4((T*)a.out + (size_t)row * a.out_ld + (size_t)head * HEAD + 4 * l,
                make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
         if (a.lse && l == 0)
             a.lse[(size_t)row * a.q_heads + head] =
-                top == -INFINITY ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+                sum == 0.f ? -INFINITY : (top + log2f(sum)) * LN2;
     }
 }
 
@@ -260,25 +254,26 @@ struct Plan {
 Plan plan_of(const jl_tree_attn& a, int sms) {
     Plan p;
     const int rows = a.max_nodes * (a.q_heads / a.pool.kv_heads);
-    p.tile_rows = rows <= 16 ? 16 : 64;
+    const bool tc = a.pool.dtype == JL_KV_BF16;
+    p.tile_rows = tc ? tc_tile_rows(a.dtype == JL_KV_F32) : rows <= 16 ? 16 : 64;
     p.lanes = (rows + p.tile_rows - 1) / p.tile_rows;
-    p.workers = std::max(1, sms / p.lanes);
+    p.workers = std::max(1, (tc ? TC_CTAS_PER_SM : 1) * sms / p.lanes);
     p.min_units = 2;
     p.bytes = p.workers == 1 ? 0 : (size_t)p.workers * p.lanes * 2 * p.tile_rows * (HEAD + 2) * sizeof(float);
     return p;
 }
 
-template <typename KV, typename T>
+template <typename T>
 jl_status launch_cc(const Args& a, cudaStream_t st) {
     const dim3 grid(a.workers, a.lanes);
-    if (a.tile_rows == 16) return launch_pdl(k_tree_attn_cc<KV, T, 1>, grid, dim3(CC_T), cc_smem<1>(), st, a);
-    return launch_pdl(k_tree_attn_cc<KV, T, 4>, grid, dim3(CC_T), cc_smem<4>(), st, a);
+    if (a.tile_rows == 16) return launch_pdl(k_tree_attn_cc<T, 1>, grid, dim3(CC_T), cc_smem<1>(), st, a);
+    return launch_pdl(k_tree_attn_cc<T, 4>, grid, dim3(CC_T), cc_smem<4>(), st, a);
 }
 
-template <typename KV, typename T>
+template <typename T>
 jl_status configure_cc() {
-    JL_CUDA(cudaFuncSetAttribute(k_tree_attn_cc<KV, T, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cc_smem<1>()));
-    JL_CUDA(cudaFuncSetAttribute(k_tree_attn_cc<KV, T, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cc_smem<4>()));
+    JL_CUDA(cudaFuncSetAttribute(k_tree_attn_cc<T, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cc_smem<1>()));
+    JL_CUDA(cudaFuncSetAttribute(k_tree_attn_cc<T, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cc_smem<4>()));
     return JL_OK;
 }
 
@@ -287,10 +282,9 @@ jl_status configure(int device) {  // once per device
     static bool done[64] = {};
     std::lock_guard<std::mutex> g(mu);
     if (device < 64 && done[device]) return JL_OK;
-    JL_TRY((configure_cc<float, float>()));
-    JL_TRY((configure_cc<float, uint16_t>()));
-    JL_TRY((configure_cc<uint16_t, float>()));
-    JL_TRY((configure_cc<uint16_t, uint16_t>()));
+    JL_TRY((configure_cc<float>()));
+    JL_TRY((configure_cc<uint16_t>()));
+    JL_TRY(tc_configure());
     if (device < 64) done[device] = true;
     return JL_OK;
 }
@@ -360,8 +354,8 @@ jl_status tree_attention(const jl_tree_attn& a, cudaStream_t st) {
     k.ws_ml = k.ws_o + (size_t)p.workers * p.lanes * 2 * p.tile_rows * HEAD;
     k.status = a.status;
     const bool f = a.dtype == JL_KV_F32;
-    if (a.pool.dtype == JL_KV_F32) JL_TRY((f ? launch_cc<float, float>(k, st) : launch_cc<float, uint16_t>(k, st)));
-    else JL_TRY((f ? launch_cc<uint16_t, float>(k, st) : launch_cc<uint16_t, uint16_t>(k, st)));
+    if (a.pool.dtype == JL_KV_BF16) JL_TRY(tc_launch(k, f, st));
+    else JL_TRY((f ? launch_cc<float>(k, st) : launch_cc<uint16_t>(k, st)));
     if (p.workers > 1) {
         // enough blocks that a tile's rows are added at once
         const dim3 grid(p.workers - 1, p.lanes, std::max(1, p.tile_rows / (CB_T / 32)));

@@ -90,15 +90,17 @@ __device__ __forceinline__ Split split_of(const Args& a, long long total) {
     return s;
 }
 
+struct LocateScratch {  // in shared memory
+    long long sum[16];
+    long long first;
+    int s;
+};
+
 // Finds the sequence that unit `at(w)` lies in.  Called by all `T` threads of
 // the block (a multiple of 32, at most 512); returns the split and leaves the
 // sequence and its first unit in *s, *first (s == seqs: no work).
 template <int T>
-__device__ __forceinline__ Split locate(const Args& a, int w, int* s, long long* first) {
-    __shared__ long long part[T];
-    __shared__ long long wsum[T / 32];
-    __shared__ long long found_first;
-    __shared__ int found_s;
+__device__ __forceinline__ Split locate(const Args& a, int w, LocateScratch& sc, int* s, long long* first) {
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int per = (a.seqs + T - 1) / T;
     const int s0 = min(a.seqs, t * per), s1 = min(a.seqs, s0 + per);
@@ -110,36 +112,33 @@ __device__ __forceinline__ Split locate(const Args& a, int w, int* s, long long*
         const long long up = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += up;
     }
-    if (lane == 31) wsum[warp] = inc;
+    if (lane == 31) sc.sum[warp] = inc;
     if (t == 0) {
-        found_s = a.seqs;
-        found_first = 0;
+        sc.s = a.seqs;
+        sc.first = 0;
     }
-    part[t] = inc - mine;
     __syncthreads();
-    long long base = 0, total = 0;
+    long long from = inc - mine, total = 0;
 #pragma unroll
     for (int i = 0; i < T / 32; ++i) {
-        if (i < warp) base += wsum[i];
-        total += wsum[i];
+        if (i < warp) from += sc.sum[i];
+        total += sc.sum[i];
     }
     const Split sp = split_of(a, total);
-    const long long u = sp.at(w), from = base + part[t];
+    const long long u = sp.at(w);
     if (mine > 0 && u >= from && u < from + mine) {
-        long long f = from;
         int i = s0;
-        for (;;) {
+        for (;; ++i) {
             const long long len = (long long)a.kv_heads * seq_of(a, i).np;
-            if (u < f + len) break;
-            f += len;
-            ++i;
+            if (u < from + len) break;
+            from += len;
         }
-        found_s = i;
-        found_first = f;
+        sc.s = i;
+        sc.first = from;
     }
     __syncthreads();
-    *s = found_s;
-    *first = found_first;
+    *s = sc.s;
+    *first = sc.first;
     return sp;
 }
 
@@ -202,6 +201,22 @@ __device__ __forceinline__ uint64_t visible(const Args& a, const Seq& q, int nod
     }
     return v;
 }
+
+// 2^x (ex2.approx.ftz: relative error about 2^-22, results below 2^-126 zero).
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+constexpr float LN2 = 0.6931471805599453f;
+
+// Tensor-core kernel (tree_attn_tc.cu): query rows of a tile, CTAs per SM, and
+// the launch over a pool of bf16 pages; `f32`: the type of the q and out rows.
+constexpr int TC_CTAS_PER_SM = 2;
+constexpr int tc_tile_rows(bool f32) { return f32 ? 64 : 128; }
+jl_status tc_configure();
+jl_status tc_launch(const Args& a, bool f32, cudaStream_t st);
 
 }  // namespace tree
 }  // namespace jl

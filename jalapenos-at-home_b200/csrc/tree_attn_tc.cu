@@ -1,0 +1,545 @@
+// Tree attention on tensor cores, for pools of bf16 pages.
+//
+// A CTA walks its worker's range (tree_attn.cuh) page by page with six warps:
+// warp 5 brings K and V pages into two rings by TMA, warp 4 issues the MMAs,
+// and warps 0-3 do the softmax, a thread per query row (MMA row = TMEM lane).
+//   * S = Q K^T (128 x 64 f32) goes to TMEM.  Queries are exact in bf16; f32
+//     queries enter as three bf16 pieces (24 bits), smallest first.
+//   * The softmax thread reads its row's 64 scores, masks those it does not
+//     see (only on pages past the committed positions), and writes the weights
+//     2^(s c2 - m) back over the scores as bf16 pieces (two for bf16 outputs,
+//     which leaves 2^-17, and three for f32): the A operand of the next MMA.
+//   * O += P V accumulates in TMEM over the whole segment.  m is the maximum
+//     when it was last moved: it moves, and O is rescaled, only when a row's
+//     maximum has grown by more than 2^8, so that pages seldom touch O.
+//   * With bf16 rows the scores of page j + 1 are computed while page j's
+//     weights are (two S buffers).  Three pieces fill that space, so f32 rows
+//     take one buffer and leave the overlap to the second CTA of the SM.
+// Sums, maxima and O are f32.  V rows past the sequence, and values of tree
+// nodes that are not finite, are cleared in shared memory before P V (zero
+// times them would be NaN in rows that do not see them); rows that do see such
+// a value get it added from global memory at the end.
+// A page outside the pool is read as rows past the end of the tensor map,
+// which arrive as zeros, and masked.
+#include <cuda.h>
+#include <cuda_bf16.h>
+
+#include "kernels.cuh"
+#include "launch.cuh"
+#include "mx_pieces.cuh"
+#include "ptx.cuh"
+#include "tree_attn.cuh"
+
+namespace jl {
+namespace tree {
+namespace {
+
+using mx::swz128;
+
+constexpr int T_THREADS = 192;
+constexpr int W_MMA = 4, W_TMA = 5;
+constexpr uint32_t PAGE_BYTES = PAGE * HEAD * 2;  // one head's K or V of a page: two boxes of 64 dims
+constexpr uint32_t BOX_BYTES = PAGE_BYTES / 2;
+constexpr uint32_t COL_O = 128, TMEM_COLS = 256;
+constexpr uint32_t WAIT_POLLS = 1u << 20;
+constexpr float MOVE = 8.f;  // log2 of how far a row's maximum may grow before it is moved
+
+template <typename T>
+struct Cfg;
+template <>
+struct Cfg<uint16_t> {
+    static constexpr int ROWS = tc_tile_rows(false), NQ = 1, NP = 2, SB = 2, NK = 3, NV = 2;
+};
+template <>
+struct Cfg<float> {
+    // 64 rows: three pieces of them take 48 KB, which leaves two CTAs an SM
+    static constexpr int ROWS = tc_tile_rows(true), NQ = 3, NP = 3, SB = 1, NK = 2, NV = 2;
+};
+
+template <int NK, int NV>
+struct Ctl {
+    uint64_t kfull[NK], kempty[NK], vfull[NV], vempty[NV];
+    uint64_t sfull[2], pfull[2], odone[2];  // by page parity
+    uint64_t qfull, drain;
+    uint32_t tmem;
+    int stop;  // a wait gave up: every role leaves
+    LocateScratch locate;
+};
+
+template <typename T>
+constexpr uint32_t q_bytes() { return Cfg<T>::NQ * Cfg<T>::ROWS * HEAD * 2; }
+template <typename T>
+constexpr size_t tc_smem() { return q_bytes<T>() + (size_t)(Cfg<T>::NK + Cfg<T>::NV) * PAGE_BYTES + 1024; }
+static_assert(sizeof(Ctl<3, 2>) <= 1024, "control block");
+
+// Waits for a phase, for WAIT_POLLS polls or until another role stops.
+__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volatile int* stop) {
+    for (uint32_t i = 0; i < WAIT_POLLS; ++i) {
+        if (ptx::mbar_try_wait(bar, parity)) return true;
+        if ((i & 63) == 63 && *stop) return false;
+    }
+    *stop = 1;
+    return false;
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float lo_f(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float hi_f(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+
+// Query rows of a tile into shared memory as bf16 pieces, by the 128 softmax
+// threads: [piece][64-dim block][row][128 B], swizzled.
+__device__ __forceinline__ void load_q(const Args& a, const Walk& w, int row0, int live, uint8_t* sm, int tid, const uint16_t*) {
+    constexpr int R = Cfg<uint16_t>::ROWS;
+#pragma unroll 4
+    for (int i = tid; i < live * 16; i += 128) {
+        const int r = i >> 4, c = i & 15, g = row0 + r;
+        const uint4 v = *(const uint4*)((const uint16_t*)a.q + (size_t)(w.q.lo + g / a.group) * a.q_ld +
+                                        (size_t)(w.h * a.group + g % a.group) * HEAD + 8 * c);
+        *(uint4*)(sm + (c >> 3) * (R * 128) + swz128((uint32_t)r, (uint32_t)(c & 7) * 16)) = v;
+    }
+}
+__device__ __forceinline__ void load_q(const Args& a, const Walk& w, int row0, int live, uint8_t* sm, int tid, const float*) {
+    constexpr int R = Cfg<float>::ROWS;
+#pragma unroll 4
+    for (int i = tid; i < live * 32; i += 128) {
+        const int r = i >> 5, c = i & 31, g = row0 + r;
+        float4 v = *(const float4*)((const float*)a.q + (size_t)(w.q.lo + g / a.group) * a.q_ld +
+                                    (size_t)(w.h * a.group + g % a.group) * HEAD + 4 * c);
+        uint8_t* dst = sm + (c >> 4) * (R * 128) + swz128((uint32_t)r, (uint32_t)(c & 15) * 8);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+            const uint32_t x = pack_bf16(v.x, v.y), y = pack_bf16(v.z, v.w);
+            *(uint2*)(dst + p * (2 * R * 128)) = make_uint2(x, y);
+            v = make_float4(v.x - lo_f(x), v.y - hi_f(x), v.z - lo_f(y), v.w - hi_f(y));
+        }
+    }
+}
+
+// S = Q K^T of one page, pieces smallest first.
+template <typename T>
+__device__ __forceinline__ void issue_scores(uint32_t q, uint32_t k, uint32_t tmem_s) {
+    constexpr uint32_t blk = Cfg<T>::ROWS * 128;
+    const uint32_t idesc = ptx::bf16_idesc(128, PAGE);
+#pragma unroll
+    for (int p = Cfg<T>::NQ - 1; p >= 0; --p)
+#pragma unroll
+        for (int db = 0; db < 2; ++db)
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                ptx::mma_bf16(tmem_s, ptx::smem_desc(q + (2 * p + db) * blk + 32 * s, 16, 1024, 2),
+                              ptx::smem_desc(k + db * BOX_BYTES + 32 * s, 16, 1024, 2), idesc,
+                              (p < Cfg<T>::NQ - 1 || db || s) ? 1u : 0u);
+}
+
+// Columns of piece p of the weights.  Two pieces: over the buffer's scores.
+// Three: behind them, the last over their first half.
+template <typename T>
+__device__ __forceinline__ uint32_t piece_col(int p) {
+    if (Cfg<T>::NP == 2) return 32u * p;
+    return p < 2 ? 64u + 32u * p : 0u;
+}
+
+// O += P V of one page: P from TMEM, V as an MN-major operand (64-dim blocks
+// BOX_BYTES apart, groups of 8 keys 1024 bytes apart).
+template <typename T>
+__device__ __forceinline__ void issue_pv(uint32_t tmem_p, uint32_t v, uint32_t tmem_o, bool first) {
+    const uint32_t idesc = ptx::bf16_idesc(128, HEAD) | (1u << 16);
+#pragma unroll
+    for (int p = Cfg<T>::NP - 1; p >= 0; --p)
+#pragma unroll
+        for (int s = 0; s < 4; ++s)  // keys 16 s ..
+            ptx::mma_bf16_ta(tmem_o, tmem_p + piece_col<T>(p) + 8 * s, ptx::smem_desc(v + 2048 * s, BOX_BYTES, 1024, 2),
+                             idesc, (p < Cfg<T>::NP - 1 || s || !first) ? 1u : 0u);
+}
+
+__device__ __forceinline__ bool odd_bf16(uint32_t h) { return (h & 0x7f80u) == 0x7f80u; }  // infinite or NaN
+
+// Clears rows of a V page that lie past the sequence, and values of the tree's
+// rows that are not finite; true if there was one of those.  Thread t of 128:
+// row t / 2, dims of block t % 2.
+__device__ __forceinline__ bool clean_v(uint8_t* v, int tree_row, int used, int t) {
+    bool odd = false;
+    const int r = t >> 1;
+    uint8_t* row = v + (t & 1) * BOX_BYTES + r * 128;
+    if (r >= used) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) *(uint4*)(row + 16 * c) = make_uint4(0u, 0u, 0u, 0u);
+    } else if (r >= tree_row) {
+        for (int c = 0; c < 8; ++c) {
+            uint4 x = *(const uint4*)(row + 16 * c);
+            uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            bool hit = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (odd_bf16(w[i])) w[i] &= 0xffff0000u, hit = true;
+                if (odd_bf16(w[i] >> 16)) w[i] &= 0x0000ffffu, hit = true;
+            }
+            if (hit) {
+                *(uint4*)(row + 16 * c) = make_uint4(w[0], w[1], w[2], w[3]);
+                odd = true;
+            }
+        }
+    }
+    return odd;
+}
+
+// Adds what clean_v took out to a warp's rows of O: for every node of this
+// segment's pages that a row sees, its weight times the values that are not
+// finite.  Arguments by value: nothing of the caller's moves to the stack.
+template <typename T>
+__device__ __noinline__ void add_odd(const Args a, const Walk w, int g, bool mine, float m, uint32_t t_o) {
+    const int32_t* pt = a.page_table + (size_t)w.s * a.max_pages;
+    const int node = g / a.group;
+    const T* q = (const T*)a.q + (size_t)(w.q.lo + (mine ? node : 0)) * a.q_ld + (size_t)(w.h * a.group + g % a.group) * HEAD;
+#pragma unroll 1
+    for (int d0 = 0; d0 < HEAD; d0 += 32) {
+        float o[32];
+        uint32_t bits[32];
+        ptx::tmem_ld32_sync(t_o + d0, o);
+        for (int p = max(w.p0, w.q.ctx / PAGE); mine && p < w.p1; ++p) {
+            const int page = pt[p];
+            if ((unsigned)page >= (unsigned)a.pages) continue;
+            const uint64_t vis = visible(a, w.q, node, p);
+            for (int r = 0; r < PAGE; ++r) {
+                const long long pos = (long long)p * PAGE + r;
+                if (!(vis >> r & 1) || pos < w.q.ctx) continue;
+                const uint16_t* k = (const uint16_t*)a.k + kv_index(page, w.h, r, a.kv_heads);
+                const uint16_t* v = (const uint16_t*)a.v + kv_index(page, w.h, r, a.kv_heads) + d0;
+                float weight = -1.f;
+#pragma unroll
+                for (int d = 0; d < 32; ++d) {
+                    if (!odd_bf16(v[d])) continue;
+                    if (weight < 0.f) {
+                        float s = 0.f;
+                        for (int e = 0; e < HEAD; ++e) {
+                            const float x = sizeof(T) == 4 ? ((const float*)q)[e] : bf16f(((const uint16_t*)q)[e]);
+                            s = fmaf(x, bf16f(k[e]), s);
+                        }
+                        weight = ex2(fmaf(s, a.c2, -m));
+                    }
+                    o[d] += weight * bf16f(v[d]);
+                }
+            }
+        }
+        __syncwarp();
+#pragma unroll
+        for (int d = 0; d < 32; ++d) bits[d] = __float_as_uint(o[d]);
+        ptx::tmem_st32(t_o + d0, bits);
+    }
+    ptx::tmem_wait_st();
+}
+
+// A barrier of the 128 softmax threads that tells whether `ok` holds for all.
+__device__ __forceinline__ bool all_of_softmax(bool ok) {
+    uint32_t r;
+    asm volatile(
+        "{\n .reg .pred p, q;\n"
+        " setp.ne.u32 p, %1, 0;\n"
+        " barrier.cta.red.and.pred q, 1, 128, p;\n"
+        " selp.u32 %0, 1, 0, q;\n}"
+        : "=r"(r)
+        : "r"((uint32_t)ok)
+        : "memory");
+    return r != 0;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_row32(T* dst, const float (&o)[32], float f);
+template <>
+__device__ __forceinline__ void store_row32<float>(float* dst, const float (&o)[32], float f) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 4)
+        *(float4*)(dst + i) = make_float4(o[i] * f, o[i + 1] * f, o[i + 2] * f, o[i + 3] * f);
+}
+template <>
+__device__ __forceinline__ void store_row32<uint16_t>(uint16_t* dst, const float (&o)[32], float f) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 8)
+        *(uint4*)(dst + i) = make_uint4(pack_bf16(o[i] * f, o[i + 1] * f), pack_bf16(o[i + 2] * f, o[i + 3] * f),
+                                        pack_bf16(o[i + 4] * f, o[i + 5] * f), pack_bf16(o[i + 6] * f, o[i + 7] * f));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
+    k_tree_attn_tc(Args a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+    constexpr int ROWS = Cfg<T>::ROWS, SB = Cfg<T>::SB, NK = Cfg<T>::NK, NV = Cfg<T>::NV, NP = Cfg<T>::NP;
+    extern __shared__ __align__(1024) uint8_t sm[];
+    uint8_t* kring = sm + q_bytes<T>();
+    uint8_t* vring = kring + NK * PAGE_BYTES;
+    Ctl<NK, NV>& ctl = *(Ctl<NK, NV>*)(vring + NV * PAGE_BYTES);
+    volatile int* stop = &ctl.stop;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int worker = blockIdx.x, tile = blockIdx.y;
+    if (tid == 0) {
+        for (int i = 0; i < NK; ++i) {
+            ptx::mbar_init(&ctl.kfull[i], 1);
+            ptx::mbar_init(&ctl.kempty[i], 1);
+        }
+        for (int i = 0; i < NV; ++i) {
+            ptx::mbar_init(&ctl.vfull[i], 1);
+            ptx::mbar_init(&ctl.vempty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            ptx::mbar_init(&ctl.sfull[i], 1);
+            ptx::mbar_init(&ctl.pfull[i], 4);
+            ptx::mbar_init(&ctl.odone[i], 1);
+        }
+        ptx::mbar_init(&ctl.qfull, 4);
+        ptx::mbar_init(&ctl.drain, 1);
+        ptx::fence_barrier_init();
+        ctl.stop = 0;
+        ptx::prefetch_tensormap(&kmap);
+        ptx::prefetch_tensormap(&vmap);
+    }
+    if (warp == W_MMA) {
+        ptx::tmem_alloc(&ctl.tmem, TMEM_COLS);
+        ptx::tmem_relinquish();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem = ctl.tmem;
+    ptx::grid_dependency_wait();
+    ptx::launch_dependents();
+    int s;
+    long long first;
+    const Split sp = locate<T_THREADS>(a, worker, ctl.locate, &s, &first);
+    Walk w;
+    const bool work = worker < sp.used && w.start(a, s, first, sp.at(worker), sp.at(worker + 1)) &&
+                      !(ptx::smem_u32(sm) & 1023);
+    const int row0 = tile * ROWS;
+
+    if (work && warp == W_TMA && lane == 0) {
+        const int none = a.pages * a.kv_heads * PAGE;  // the row after the pool's last
+        uint32_t it = 0;
+        bool ok = true;
+        do {
+            if (w.q.n * a.group <= row0) continue;
+            const int32_t* pt = a.page_table + (size_t)w.s * a.max_pages;
+            for (int p = w.p0; ok && p < w.p1; ++p, ++it) {
+                const int page = pt[p];
+                const bool there = (unsigned)page < (unsigned)a.pages;
+                if (!there) flag(a.status, ST_PAGE);
+                const int y = there ? (page * a.kv_heads + w.h) * PAGE : none;
+                const uint32_t ks = it % NK, vs = it % NV;
+                if (!wait_phase(&ctl.kempty[ks], (it / NK + 1) & 1, stop)) ok = false;
+                if (ok) {
+                    ptx::mbar_arrive_expect_tx(&ctl.kfull[ks], PAGE_BYTES);
+                    ptx::tma_load_2d(kring + ks * PAGE_BYTES, &kmap, 0, y, &ctl.kfull[ks]);
+                    ptx::tma_load_2d(kring + ks * PAGE_BYTES + BOX_BYTES, &kmap, 64, y, &ctl.kfull[ks]);
+                    if (!wait_phase(&ctl.vempty[vs], (it / NV + 1) & 1, stop)) {
+                        ok = false;
+                        ptx::mbar_wait(&ctl.kfull[ks], (it / NK) & 1, WAIT_POLLS);
+                    }
+                }
+                if (ok) {
+                    ptx::mbar_arrive_expect_tx(&ctl.vfull[vs], PAGE_BYTES);
+                    ptx::tma_load_2d(vring + vs * PAGE_BYTES, &vmap, 0, y, &ctl.vfull[vs]);
+                    ptx::tma_load_2d(vring + vs * PAGE_BYTES + BOX_BYTES, &vmap, 64, y, &ctl.vfull[vs]);
+                }
+            }
+        } while (ok && w.next(a));
+        // every copy in flight lands before the shared memory is given up
+        for (uint32_t i = it > NK ? it - NK : 0; i < it; ++i) ptx::mbar_wait(&ctl.kfull[i % NK], (i / NK) & 1, WAIT_POLLS);
+        for (uint32_t i = it > NV ? it - NV : 0; i < it; ++i) ptx::mbar_wait(&ctl.vfull[i % NV], (i / NV) & 1, WAIT_POLLS);
+    } else if (work && warp == W_MMA && lane == 0) {
+        const uint32_t q = ptx::smem_u32(sm), kr = ptx::smem_u32(kring), vr = ptx::smem_u32(vring);
+        uint32_t it = 0, seg = 0;
+        bool ok = true;
+        auto scores = [&](uint32_t i) {
+            ok = wait_phase(&ctl.kfull[i % NK], (i / NK) & 1, stop);
+            if (!ok) return;
+            ptx::tc_fence_after();
+            issue_scores<T>(q, kr + (i % NK) * PAGE_BYTES, tmem + 64 * (i % SB));
+            ptx::tc_commit(&ctl.kempty[i % NK]);
+            ptx::tc_commit(&ctl.sfull[i & 1]);
+        };
+        do {
+            if (w.q.n * a.group <= row0) continue;
+            const int n = w.p1 - w.p0;
+            ok = wait_phase(&ctl.qfull, seg++ & 1, stop);
+            if (ok) scores(it);
+            for (int i = 0; ok && i < n; ++i, ++it) {
+                if (SB == 2 && i + 1 < n) scores(it + 1);
+                ok = ok && wait_phase(&ctl.pfull[it & 1], (it >> 1) & 1, stop) &&
+                     wait_phase(&ctl.vfull[it % NV], (it / NV) & 1, stop);
+                if (!ok) break;
+                ptx::tc_fence_after();
+                issue_pv<T>(tmem + 64 * (it % SB), vr + (it % NV) * PAGE_BYTES, tmem + COL_O, i == 0);
+                ptx::tc_commit(&ctl.vempty[it % NV]);
+                ptx::tc_commit(&ctl.odone[it & 1]);
+                if (SB == 1 && i + 1 < n) scores(it + 1);
+            }
+        } while (ok && w.next(a));
+        // every MMA is done before TMEM and the shared memory are given up
+        ptx::tc_commit(&ctl.drain);
+        ptx::mbar_wait(&ctl.drain, 0, WAIT_POLLS);
+    } else if (work && warp < 4) {
+        const uint32_t t_lane = tmem + ((uint32_t)(warp * 32) << 16);
+        uint32_t it = 0;
+        bool ok = true;
+        do {
+            const int live = min(ROWS, w.q.n * a.group - row0);
+            if (live <= 0) continue;
+            const int g = row0 + tid, n = w.p1 - w.p0;
+            const bool mine = tid < live, active = warp * 32 < live;
+            load_q(a, w, row0, live, sm, tid, (const T*)nullptr);
+            ptx::fence_proxy_async_smem();
+            ptx::tc_fence_before();  // and the last segment's reads of O are done
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&ctl.qfull);
+            const int32_t* pt = a.page_table + (size_t)w.s * a.max_pages;
+            float m = -INFINITY, l = 0.f;
+            bool odd = false;  // this thread took a value out
+            for (int i = 0; ok && i < n; ++i, ++it) {
+                const int p = w.p0 + i;
+                const int page = pt[p];
+                const bool there = (unsigned)page < (unsigned)a.pages;
+                const bool edge = !there || (long long)(p + 1) * PAGE > w.q.ctx;
+                if (edge) {
+                    ok = wait_phase(&ctl.vfull[it % NV], (it / NV) & 1, stop);
+                    if (ok) {
+                        const long long left = (long long)w.q.ctx + w.q.n - (long long)p * PAGE;
+                        odd |= clean_v(vring + (it % NV) * PAGE_BYTES, max(0, (int)min(64ll, w.q.ctx - (long long)p * PAGE)),
+                                       there ? (int)min(64ll, left) : 0, tid);
+                        ptx::fence_proxy_async_smem();
+                    }
+                }
+                ok = ok && wait_phase(&ctl.sfull[it & 1], (it >> 1) & 1, stop);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                ptx::tc_fence_after();
+                if (active) {
+                    const uint32_t t_s = t_lane + 64 * (it % SB);
+                    float x[64];
+                    ptx::tmem_ld64_sync(t_s, x);
+                    if (edge) {
+                        const uint64_t vis = mine && there ? visible(a, w.q, g / a.group, p) : 0;
+                        const uint32_t v0 = (uint32_t)vis, v1 = (uint32_t)(vis >> 32);
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) {
+                            if (!(v0 >> c & 1)) x[c] = -INFINITY;
+                            if (!(v1 >> c & 1)) x[32 + c] = -INFINITY;
+                        }
+                    }
+                    float t0 = fmaxf(x[0], x[1]), t1 = fmaxf(x[2], x[3]);
+#pragma unroll
+                    for (int c = 4; c < 64; c += 4) {
+                        t0 = fmaxf(t0, fmaxf(x[c], x[c + 1]));
+                        t1 = fmaxf(t1, fmaxf(x[c + 2], x[c + 3]));
+                    }
+                    const float top = fmaxf(t0, t1) * a.c2;
+                    float f = 1.f;
+                    if (m == -INFINITY) {
+                        m = top;  // nothing was seen before: O and l are zero
+                    } else if (top > m + MOVE) {
+                        f = ex2(m - top);
+                        m = top;
+                        l *= f;
+                    }
+                    if (i > 0 && __any_sync(0xffffffffu, mine && f != 1.f)) {
+                        const uint32_t j = it - 1;  // every earlier P V is done
+                        ok = __all_sync(0xffffffffu, wait_phase(&ctl.odone[j & 1], (j >> 1) & 1, stop));
+                        if (!ok) break;
+                        ptx::tc_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < HEAD; c += 32) {
+                            float o[32];
+                            uint32_t r[32];
+                            ptx::tmem_ld32_sync(t_lane + COL_O + c, o);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(o[e] * f);
+                            ptx::tmem_st32(t_lane + COL_O + c, r);
+                        }
+                    }
+                    const float ref = m == -INFINITY ? 0.f : m;
+                    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+                    for (int c = 0; c < 64; c += 2) {
+                        x[c] = ex2(fmaf(x[c], a.c2, -ref));
+                        x[c + 1] = ex2(fmaf(x[c + 1], a.c2, -ref));
+                        s0 += x[c];
+                        s1 += x[c + 1];
+                    }
+                    l += s0 + s1;
+#pragma unroll
+                    for (int pc = 0; pc < NP; ++pc) {
+                        uint32_t r[32];
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) {
+                            r[c] = pack_bf16(x[2 * c], x[2 * c + 1]);
+                            if (pc + 1 < NP) {
+                                x[2 * c] -= lo_f(r[c]);
+                                x[2 * c + 1] -= hi_f(r[c]);
+                            }
+                        }
+                        ptx::tmem_st32(t_s + piece_col<T>(pc), r);
+                    }
+                    ptx::tmem_wait_st();
+                }
+                ptx::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(&ctl.pfull[it & 1]);
+            }
+            if (ok) {
+                const uint32_t j = it - 1;
+                ok = wait_phase(&ctl.odone[j & 1], (j >> 1) & 1, stop);
+            }
+            ok = all_of_softmax(ok);
+            if (!ok) break;
+            ptx::tc_fence_after();
+            odd = !all_of_softmax(!odd);
+            if (active) {
+                if (odd) add_odd<T>(a, w, g, mine, m == -INFINITY ? 0.f : m, t_lane + COL_O);
+                const bool whole = w.whole();
+                const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);  // 0: nothing seen
+                const size_t part = (((size_t)worker * a.lanes + tile) * 2 + w.slot()) * ROWS + tid;
+                const int row = w.q.lo + g / a.group, head = w.h * a.group + g % a.group;
+#pragma unroll 1
+                for (int c = 0; c < HEAD; c += 32) {
+                    float o[32];
+                    ptx::tmem_ld32_sync(t_lane + COL_O + c, o);
+                    if (mine) {
+                        if (whole) store_row32<T>((T*)a.out + (size_t)row * a.out_ld + (size_t)head * HEAD + c, o, inv);
+                        else store_row32<float>(a.ws_o + part * HEAD + c, o, 1.f);
+                    }
+                }
+                if (mine && whole && a.lse) a.lse[(size_t)row * a.q_heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+                if (mine && !whole) *(float2*)(a.ws_ml + part * 2) = make_float2(m, l);
+            }
+        } while (w.next(a));
+    }
+    __syncwarp();
+    __syncthreads();
+    if (tid == 0 && (ctl.stop || (ptx::smem_u32(sm) & 1023))) flag(a.status, ST_TIMEOUT);
+    ptx::tc_fence_after();
+    if (warp == W_MMA) ptx::tmem_dealloc(tmem, TMEM_COLS);
+}
+
+template <typename T>
+jl_status launch(const Args& a, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st) {
+    return launch_pdl(k_tree_attn_tc<T>, dim3(a.workers, a.lanes), dim3(T_THREADS), tc_smem<T>(), st, a, k, v);
+}
+
+}  // namespace
+
+jl_status tc_configure() {
+    JL_CUDA(cudaFuncSetAttribute(k_tree_attn_tc<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tc_smem<float>()));
+    JL_CUDA(cudaFuncSetAttribute(k_tree_attn_tc<uint16_t>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 (int)tc_smem<uint16_t>()));
+    return JL_OK;
+}
+
+jl_status tc_launch(const Args& a, bool f32, cudaStream_t st) {
+    const uint64_t rows = (uint64_t)a.pages * a.kv_heads * PAGE;
+    CUtensorMap k, v;
+    JL_TRY(kv_page_map(&k, const_cast<void*>(a.k), rows));
+    JL_TRY(kv_page_map(&v, const_cast<void*>(a.v), rows));
+    return f32 ? launch<float>(a, k, v, st) : launch<uint16_t>(a, k, v, st);
+}
+
+}  // namespace tree
+}  // namespace jl
