@@ -459,26 +459,44 @@ bool prefill_tc_supported(const jl_model* m) {
     return group == 1 || group == 2 || group == 4 || group == 8;
 }
 
-// The TMA view of one layer's K or V pages: rows (page, kv head, slot) of HEAD
-// bf16, boxes of 64 dims x one page, 128-byte swizzle.
-jl_status kv_page_map(CUtensorMap* map, void* pages, uint64_t rows) {
+namespace {
+// A tensor of bf16 with a dense innermost dimension of HEAD, read in boxes of
+// 64 of its elements with 128-byte swizzle.
+jl_status bf16_map(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+                   const cuuint32_t* box) {
     PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
     if (!enc) {
         set_error("cuTensorMapEncodeTiled is not available from the driver");
         return JL_ERR_CUDA;
     }
-    const cuuint64_t dims[2] = {(cuuint64_t)HEAD, (cuuint64_t)rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)HEAD * 2};
-    const cuuint32_t box[2] = {64, (cuuint32_t)PAGE};
-    const cuuint32_t es[2] = {1, 1};
-    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, pages, dims, strides, box, es,
+    const cuuint32_t es[3] = {1, 1, 1};
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides, box, es,
                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
-        set_error("cuTensorMapEncodeTiled failed (%d) for KV pages at %p", (int)r, pages);
+        set_error("cuTensorMapEncodeTiled failed (%d) for a tensor at %p", (int)r, base);
         return JL_ERR_CUDA;
     }
     return JL_OK;
+}
+}  // namespace
+
+// The TMA view of one layer's K or V pages: rows (page, kv head, slot) of HEAD
+// bf16, boxes of 64 dims x one page.
+jl_status kv_page_map(CUtensorMap* map, const void* pages, uint64_t rows) {
+    const cuuint64_t dims[2] = {(cuuint64_t)HEAD, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)HEAD * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)PAGE};
+    return bf16_map(map, pages, 2, dims, strides, box);
+}
+
+// The TMA view of bf16 query rows [rows][heads][HEAD], ld elements apart:
+// boxes of 64 dims x `box_heads` heads x `box_rows` rows.
+jl_status q_row_map(CUtensorMap* map, const void* q, int heads, int rows, long long ld, int box_heads, int box_rows) {
+    const cuuint64_t dims[3] = {(cuuint64_t)HEAD, (cuuint64_t)heads, (cuuint64_t)rows};
+    const cuuint64_t strides[2] = {(cuuint64_t)HEAD * 2, (cuuint64_t)ld * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_rows};
+    return bf16_map(map, q, 3, dims, strides, box);
 }
 
 // Two tensor maps per layer over its K and V pages.

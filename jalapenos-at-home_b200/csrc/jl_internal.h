@@ -328,7 +328,8 @@ jl_status record_pass_ctx(const PassCtx& c, int layers, bool with_head);
 jl_status configure_kernels();
 // Tensor-core prompt attention (attn_prefill_tc.cu).
 jl_status kv_tensor_maps(jl_model* m);
-jl_status kv_page_map(CUtensorMap* map, void* pages, uint64_t rows);
+jl_status kv_page_map(CUtensorMap* map, const void* pages, uint64_t rows);
+jl_status q_row_map(CUtensorMap* map, const void* q, int heads, int rows, long long ld, int box_heads, int box_rows);
 jl_status configure_prefill_tc();
 bool prefill_tc_supported(const jl_model* m);
 jl_status launch_attention_prefill_tc(const PassCtx& c, int layer, uint8_t* bout, int bN);

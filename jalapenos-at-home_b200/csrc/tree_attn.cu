@@ -55,11 +55,11 @@ __global__ void __launch_bounds__(CC_T) k_tree_attn_cc(Args a) {
     ptx::grid_dependency_wait();
     ptx::launch_dependents();
     __shared__ LocateScratch scratch;
-    int s;
-    long long first;
-    const Split sp = locate<CC_T>(a, worker, scratch, &s, &first);
+    const Split sp = locate<CC_T>(a, worker, scratch);
     Walk w;
-    if (worker >= sp.used || !w.start(a, s, first, sp.at(worker), sp.at(worker + 1))) return;
+    const bool work = w.start(a, scratch.found, sp.at(worker), sp.at(worker + 1));
+    if (tid == 0 && lane == 0 && a.workers > 1) a.ws_join[worker] = w.join(sp, worker, work);
+    if (!work) return;
     do {
         const int live = min(R, w.q.n * a.group - lane * R);  // rows of this tile
         if (live <= 0) continue;
@@ -188,58 +188,160 @@ __global__ void __launch_bounds__(CC_T) k_tree_attn_cc(Args a) {
 
 // ---- partial results -----------------------------------------------------------------
 //
-// Block (w, lane, z): if worker w's range starts inside an item and is the
-// first to do so, the item's partials, from worker w - 1 on, are added in
-// order: a warp per row, lane l holding dims 4 l ...  z deals the rows out.
-constexpr int CB_T = 256;
+// The rows to add (query rows of the items that ws_join names) are dealt out
+// over all blocks: each block scans the at most CB_MOST entries into a list of
+// items and the groups of rows before each, then takes every gridDim.x-th
+// group.  Lane l of a warp holds dims 4 l .. of a row.  An item of few partials
+// has groups of CB_ROWS rows, CB_ROWS / CB_WARPS of them to a warp at once; one
+// of many has groups of one row, whose partials the warps share and add in
+// order.
+constexpr int CB_WARPS = 4, CB_T = 32 * CB_WARPS;
+constexpr int CB_MOST = 512;   // workers at most
+constexpr int CB_SHARE = 8;    // partials from which the warps share a row
+constexpr int CB_AHEAD = 8;    // loads in flight
+constexpr int CB_ROWS = 16, CB_RPW = CB_ROWS / CB_WARPS;
+
+struct RowSum {
+    float top, sum;
+    float4 o;
+};
+__device__ __forceinline__ void add_part(RowSum& t, float m, float l, float4 v) {
+    if (l == 0.f) return;  // nothing seen there
+    const float top = fmaxf(t.top, m), ref = top == -INFINITY ? 0.f : top;
+    const float f = ex2(t.top - ref), g = ex2(m - ref);
+    t.top = top;
+    t.sum = fmaf(t.sum, f, l * g);
+    t.o = make_float4(fmaf(t.o.x, f, v.x * g), fmaf(t.o.y, f, v.y * g), fmaf(t.o.z, f, v.z * g), fmaf(t.o.w, f, v.w * g));
+}
 
 template <typename T>
 __global__ void __launch_bounds__(CB_T) k_tree_combine(Args a) {
-    const int w = blockIdx.x + 1, lane = blockIdx.y;
-    const int warp = threadIdx.x >> 5, l = threadIdx.x & 31;
+    __shared__ float4 share_o[CB_WARPS][32];
+    __shared__ float2 share_ml[CB_WARPS];
+    __shared__ int before[CB_MOST + 1];  // groups of CB_WARPS rows before item i
+    __shared__ short who[CB_MOST];       // item i is ws_join[who[i]]
+    __shared__ int warp_items[CB_WARPS], warp_groups[CB_WARPS];
+    const int t = threadIdx.x, warp = t >> 5, l = t & 31;
     ptx::grid_dependency_wait();
     ptx::launch_dependents();
-    __shared__ LocateScratch scratch;
-    int s;
-    long long first;
-    const Split sp = locate<CB_T>(a, w, scratch, &s, &first);
-    if (w >= sp.used || s >= a.seqs) return;
-    const Seq q = seq_of(a, s);
-    const long long u = sp.at(w);
-    const int h = (int)((u - first) / q.np);
-    const long long item = first + (long long)h * q.np, item_end = item + q.np;
-    if (u == item || sp.at(w - 1) > item) return;  // starts on an item, or not the first inside it
-    int last = w;
-    while (sp.at(last + 1) < item_end) ++last;
-    const int R = a.tile_rows, live = min(R, q.n * a.group - lane * R);
-    for (int r = blockIdx.z * (CB_T / 32) + warp; r < live; r += gridDim.z * (CB_T / 32)) {
-        // worker w - 1 began the item unless its range starts exactly on it, or
-        // before it: its partial is then the one of the item its range ends in
-        auto slot = [&](int x) { return (((size_t)x * a.lanes + lane) * 2 + (x == w - 1 ? 1 : 0)) * R + r; };
-        float top = -INFINITY;
-        for (int x = w - 1 + l; x <= last; x += 32) top = fmaxf(top, a.ws_ml[slot(x) * 2]);
-        top = warp_max(top);
-        const float ref = top == -INFINITY ? 0.f : top;
-        float sum = 0.f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int x = w - 1; x <= last; ++x) {
-            const float2 ml = *(const float2*)(a.ws_ml + slot(x) * 2);
-            const float4 v = *(const float4*)(a.ws_o + slot(x) * HEAD + 4 * l);
-            const float f = ml.y == 0.f ? 0.f : ex2(ml.x - ref);  // 0: nothing seen there
-            sum = fmaf(ml.y, f, sum);
-            o.x = fmaf(v.x, f, o.x);
-            o.y = fmaf(v.y, f, o.y);
-            o.z = fmaf(v.z, f, o.z);
-            o.w = fmaf(v.w, f, o.w);
+    // items and their groups of rows, over all tiles (the last may be short)
+    int items = 0, groups = 0;
+    for (int w0 = 0; w0 < a.workers; w0 += CB_T) {
+        const int w = w0 + t;
+        const int4 join = w > 0 && w < a.workers ? a.ws_join[w] : make_int4(0, 0, 0, 0);
+        const int rows = join.w > 0 ? join.y * a.group : 0, g = join.w >= CB_SHARE ? rows : (rows + CB_ROWS - 1) / CB_ROWS;
+        const unsigned some = __ballot_sync(0xffffffffu, g > 0);
+        int inc = g;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, inc, o);
+            if (l >= o) inc += up;
         }
-        const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
-        const int g = lane * R + r, row = q.lo + g / a.group, head = h * a.group + g % a.group;
-        store4((T*)a.out + (size_t)row * a.out_ld + (size_t)head * HEAD + 4 * l,
-               make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
-        if (a.lse && l == 0)
-            a.lse[(size_t)row * a.q_heads + head] =
-                sum == 0.f ? -INFINITY : (top + log2f(sum)) * LN2;
+        if (l == 31) {
+            warp_items[warp] = __popc(some);
+            warp_groups[warp] = inc;
+        }
+        __syncthreads();
+        int at = items + __popc(some & ((1u << l) - 1)), sum = groups + inc - g;
+#pragma unroll
+        for (int i = 0; i < CB_WARPS; ++i) {
+            if (i < warp) {
+                at += warp_items[i];
+                sum += warp_groups[i];
+            }
+            items += warp_items[i];
+            groups += warp_groups[i];
+        }
+        if (g > 0) {
+            who[at] = (short)w;
+            before[at] = sum;
+        }
+        __syncthreads();
+    }
+    if (t == 0) before[items] = groups;
+    __syncthreads();
+    const float inv_group = 1.f / a.group;
+    const int R = a.tile_rows;
+    int item = 0;
+    for (int i = blockIdx.x; i < groups; i += gridDim.x) {
+        while (before[item + 1] <= i) ++item;
+        const int w = who[item];
+        const int4 join = a.ws_join[w];
+        const int rows = join.y * a.group, parts = join.w, at = i - before[item];
+        // partial x of query row g: worker w - 1's slot 1, then slot 0 of the workers from w on
+        auto slot = [&](int x, int g) {
+            const int lane = g / R;
+            return ((size_t)((w - 1 + x) * a.lanes + lane) * 2 + (x == 0 ? 1 : 0)) * R + (g - lane * R);
+        };
+        auto finish = [&](const RowSum& sum, int g) {
+            const float inv = sum.sum == 0.f ? 0.f : __fdiv_rn(1.f, sum.sum);
+            const int node = div_small(g, inv_group), head = join.z * a.group + g - node * a.group;
+            store4((T*)a.out + (size_t)(join.x + node) * a.out_ld + (size_t)head * HEAD + 4 * l,
+                   make_float4(sum.o.x * inv, sum.o.y * inv, sum.o.z * inv, sum.o.w * inv));
+            if (a.lse && l == 0)
+                a.lse[(size_t)(join.x + node) * a.q_heads + head] =
+                    sum.sum == 0.f ? -INFINITY : (sum.top + log2f(sum.sum)) * LN2;
+        };
+        if (parts < CB_SHARE) {
+            RowSum sum[CB_RPW];
+            int g[CB_RPW];
+#pragma unroll
+            for (int r = 0; r < CB_RPW; ++r) {
+                g[r] = at * CB_ROWS + r * CB_WARPS + warp;
+                sum[r] = RowSum{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+            }
+            for (int x = 0; x < parts; x += 2) {
+                float2 ml[CB_RPW][2];
+                float4 v[CB_RPW][2];
+#pragma unroll
+                for (int r = 0; r < CB_RPW; ++r)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        ml[r][e] = make_float2(-INFINITY, 0.f);
+                        v[r][e] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (x + e < parts && g[r] < rows) {
+                            const size_t p = slot(x + e, g[r]);
+                            ml[r][e] = *(const float2*)(a.ws_ml + p * 2);
+                            v[r][e] = *(const float4*)(a.ws_o + p * HEAD + 4 * l);
+                        }
+                    }
+#pragma unroll
+                for (int r = 0; r < CB_RPW; ++r)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) add_part(sum[r], ml[r][e].x, ml[r][e].y, v[r][e]);
+            }
+#pragma unroll
+            for (int r = 0; r < CB_RPW; ++r)
+                if (g[r] < rows) finish(sum[r], g[r]);
+            continue;
+        }
+        const int x0 = parts * warp / CB_WARPS, x1 = parts * (warp + 1) / CB_WARPS;
+        RowSum sum{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+        for (int x = x0; x < x1; x += CB_AHEAD) {
+            float2 ml[CB_AHEAD];
+            float4 v[CB_AHEAD];
+#pragma unroll
+            for (int e = 0; e < CB_AHEAD; ++e) {
+                ml[e] = make_float2(-INFINITY, 0.f);
+                v[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (x + e < x1) {
+                    const size_t p = slot(x + e, at);
+                    ml[e] = *(const float2*)(a.ws_ml + p * 2);
+                    v[e] = *(const float4*)(a.ws_o + p * HEAD + 4 * l);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < CB_AHEAD; ++e) add_part(sum, ml[e].x, ml[e].y, v[e]);
+        }
+        __syncthreads();  // the last row's sums were read
+        share_o[warp][l] = sum.o;
+        if (l == 0) share_ml[warp] = make_float2(sum.top, sum.sum);
+        __syncthreads();
+        if (warp != 0) continue;
+        sum = RowSum{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+#pragma unroll
+        for (int e = 0; e < CB_WARPS; ++e) add_part(sum, share_ml[e].x, share_ml[e].y, share_o[e][l]);
+        finish(sum, at);
     }
 }
 
@@ -257,9 +359,9 @@ Plan plan_of(const jl_tree_attn& a, int sms) {
     const bool tc = a.pool.dtype == JL_KV_BF16;
     p.tile_rows = tc ? tc_tile_rows(a.dtype == JL_KV_F32) : rows <= 16 ? 16 : 64;
     p.lanes = (rows + p.tile_rows - 1) / p.tile_rows;
-    p.workers = std::max(1, (tc ? TC_CTAS_PER_SM : 1) * sms / p.lanes);
-    p.min_units = 2;
-    p.bytes = p.workers == 1 ? 0 : (size_t)p.workers * p.lanes * 2 * p.tile_rows * (HEAD + 2) * sizeof(float);
+    p.workers = std::min(CB_MOST, std::max(1, (tc ? TC_CTAS_PER_SM : 1) * sms / p.lanes));
+    p.min_units = 4 + SEG;  // four pages and a start
+    p.bytes = p.workers == 1 ? 0 : (size_t)p.workers * (sizeof(int4) + (size_t)p.lanes * 2 * p.tile_rows * (HEAD + 2) * sizeof(float));
     return p;
 }
 
@@ -315,6 +417,8 @@ jl_status tree_attention(const jl_tree_attn& a, cudaStream_t st) {
     JL_REFUSE(a.mask && (long long)a.mask_words * 64 < a.max_nodes, "tree attention: %d mask words hold fewer than %d nodes",
               a.mask_words, a.max_nodes);
     JL_REFUSE(a.max_pages < 1 || a.max_pages > MAX_TABLE, "tree attention: max_pages must be 1..%d", MAX_TABLE);
+    JL_REFUSE((long long)a.seqs * a.pool.kv_heads * (a.max_pages + SEG) >= (1ll << 31),
+              "tree attention: seqs * kv heads * max_pages must stay below 2^31");
     JL_REFUSE(!(a.scale >= 0.f) || std::isinf(a.scale), "tree attention: scale must be finite and not negative");
     if (a.rows == 0 || a.seqs == 0) return JL_OK;
     DeviceOf on;
@@ -350,15 +454,17 @@ jl_status tree_attention(const jl_tree_attn& a, cudaStream_t st) {
     k.lanes = p.lanes;
     k.tile_rows = p.tile_rows;
     k.min_units = p.min_units;
-    k.ws_o = (float*)a.workspace;
+    k.ws_join = (int4*)a.workspace;
+    k.ws_o = (float*)(k.ws_join + p.workers);
     k.ws_ml = k.ws_o + (size_t)p.workers * p.lanes * 2 * p.tile_rows * HEAD;
     k.status = a.status;
     const bool f = a.dtype == JL_KV_F32;
     if (a.pool.dtype == JL_KV_BF16) JL_TRY(tc_launch(k, f, st));
     else JL_TRY((f ? launch_cc<float>(k, st) : launch_cc<uint16_t>(k, st)));
     if (p.workers > 1) {
-        // enough blocks that a tile's rows are added at once
-        const dim3 grid(p.workers - 1, p.lanes, std::max(1, p.tile_rows / (CB_T / 32)));
+        // all blocks resident, at most one per row there may be
+        const long long most = (long long)(p.workers - 1) * a.max_nodes * k.group;
+        const dim3 grid((unsigned)std::min<long long>(8ll * on.sms, most));
         JL_TRY((f ? launch_pdl(k_tree_combine<float>, grid, dim3(CB_T), 0, st, k)
                   : launch_pdl(k_tree_combine<uint16_t>, grid, dim3(CB_T), 0, st, k)));
     }

@@ -1,16 +1,19 @@
 // What the kernels of tree attention share: arguments, the split of the
 // batch's work between CTAs, visibility masks and partial results.
 //
-// Work is counted in units of one page of one KV head: sequence s has
-// kv_heads * npages(s) units, item (s, h) the npages(s) of them that head h
-// reads.  The units of the whole batch, in order (s, h, page), are cut into
-// equal ranges, one per worker, so a batch of any lengths keeps every SM busy
-// for the same time.  A worker walks the segments of its range (the part of
-// one item that lies in it); a segment that is a whole item is written to the
-// output, any other leaves a partial result (unnormalised output, maximum and
-// sum of every row) in the workspace, and k_tree_combine adds an item's
-// partials in page order.  A worker has at most two partials: the item its
-// range starts in (slot 0) and the item its range ends in (slot 1).
+// Work is counted in units of one page of one KV head: item (s, h) is what head
+// h of sequence s reads, SEG units for its start and end (queries, output) and
+// then npages(s) for its pages.  The units of the whole batch, in order
+// (s, h, page), are cut into equal ranges, one per worker, so a batch of any
+// lengths keeps every SM busy for the same time.  A worker walks the segments
+// of its range (the pages of one item that lie in it); a segment that is a
+// whole item is written to the output, any other leaves a partial result
+// (unnormalised output, maximum and sum of every row) in the workspace, and
+// k_tree_combine adds an item's partials in page order.  A worker has at most
+// two partials: the item its range starts in (slot 0) and the item its range
+// ends in (slot 1).  The first worker w whose pages start inside an item says
+// in ws_join[w] what there is to add: the partial of worker w - 1 (slot 1) and
+// those of w, w + 1 .. (slot 0).
 //
 // The query rows of an item are node * group + head of the group, cut into
 // tiles of `tile_rows`; a worker is `lanes` CTAs, one per tile, that walk the
@@ -26,6 +29,9 @@
 namespace jl {
 namespace tree {
 
+// Units of a segment's start and end: about two pages' time on a B200 (4 us
+// against 1.5 us a page with two CTAs an SM).
+constexpr int SEG = 2;
 constexpr int ST_PAGE = 1, ST_RANGE = 2, ST_TIMEOUT = 4;  // status bits
 
 struct Args {
@@ -43,9 +49,11 @@ struct Args {
     const void* k;
     const void* v;
     float c2;          // scale * log2(e)
+    int4* ws_join;     // [worker]
     float* ws_o;       // [worker][lane][slot][tile_rows][HEAD]
     float* ws_ml;      // [worker][lane][slot][tile_rows][2]: maximum (scores times c2), sum
     int workers, lanes, tile_rows, min_units;
+    int q_tma;         // the tensor-core kernel's queries come by TMA
     int32_t* status;
 };
 
@@ -75,93 +83,102 @@ __device__ __forceinline__ Seq seq_of(const Args& a, int s) {
     return q;
 }
 
-// First unit of worker w's range: the units cut evenly over the workers that
-// have at least min_units each.
+// The units (fewer than 2^31, checked on the host) cut over the workers that
+// have about min_units each: the first `more` of them get `each` + 1 units.
 struct Split {
-    long long total;
-    int used;  // workers with a range
-    __device__ long long at(int w) const { return w >= used ? total : total * w / used; }
+    int used, each, more;
+    __device__ int at(int w) const { return each * min(w, used) + min(w, more); }
+    __device__ int worker_of(int u) const {
+        const int cut = (each + 1) * more;
+        return u < cut ? u / (each + 1) : more + (u - cut) / each;
+    }
 };
-__device__ __forceinline__ Split split_of(const Args& a, long long total) {
+__device__ __forceinline__ Split split_of(const Args& a, int total) {
     Split s;
-    s.total = total;
-    const long long want = (total + a.min_units - 1) / a.min_units;
-    s.used = (int)min((long long)a.workers, max(want, 1ll));
+    s.used = min(a.workers, max((total + a.min_units - 1) / a.min_units, 1));
+    s.each = total / s.used;
+    s.more = total - s.each * s.used;
     return s;
 }
 
+__device__ __forceinline__ int units_of(const Args& a, const Seq& q) { return q.np ? a.kv_heads * (q.np + SEG) : 0; }
+
+struct Found {     // the sequence a worker's range starts in
+    Seq q;
+    int s, first;  // its index and its first unit
+};
 struct LocateScratch {  // in shared memory
-    long long sum[16];
-    long long first;
-    int s;
+    int sum[16];
+    Found found;
 };
 
-// Finds the sequence that unit `at(w)` lies in.  Called by all `T` threads of
-// the block (a multiple of 32, at most 512); returns the split and leaves the
-// sequence and its first unit in *s, *first (s == seqs: no work).
+// Finds the sequence that worker w's range starts in (found.s == seqs: none).
+// Called by all `T` threads of the block (a multiple of 32, at most 512).
 template <int T>
-__device__ __forceinline__ Split locate(const Args& a, int w, LocateScratch& sc, int* s, long long* first) {
+__device__ __forceinline__ Split locate(const Args& a, int w, LocateScratch& sc) {
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int per = (a.seqs + T - 1) / T;
     const int s0 = min(a.seqs, t * per), s1 = min(a.seqs, s0 + per);
-    long long mine = 0;
-    for (int i = s0; i < s1; ++i) mine += (long long)a.kv_heads * seq_of(a, i).np;
-    long long inc = mine;
+    Seq q{0, 0, 0, 0};
+    int mine = 0;
+    for (int i = s0; i < s1; ++i) {
+        q = seq_of(a, i);
+        mine += units_of(a, q);
+    }
+    int inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long up = __shfl_up_sync(0xffffffffu, inc, o);
+        const int up = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += up;
     }
     if (lane == 31) sc.sum[warp] = inc;
-    if (t == 0) {
-        sc.s = a.seqs;
-        sc.first = 0;
-    }
+    if (t == 0) sc.found.s = a.seqs;
     __syncthreads();
-    long long from = inc - mine, total = 0;
+    int from = inc - mine, total = 0;
 #pragma unroll
     for (int i = 0; i < T / 32; ++i) {
         if (i < warp) from += sc.sum[i];
         total += sc.sum[i];
     }
     const Split sp = split_of(a, total);
-    const long long u = sp.at(w);
+    const int u = sp.at(w);
     if (mine > 0 && u >= from && u < from + mine) {
         int i = s0;
-        for (;; ++i) {
-            const long long len = (long long)a.kv_heads * seq_of(a, i).np;
-            if (u < from + len) break;
-            from += len;
-        }
-        sc.s = i;
-        sc.first = from;
+        if (per > 1)
+            for (;; ++i) {
+                q = seq_of(a, i);
+                const int len = units_of(a, q);
+                if (u < from + len) break;
+                from += len;
+            }
+        sc.found.q = q;
+        sc.found.s = i;
+        sc.found.first = from;
     }
     __syncthreads();
-    *s = sc.s;
-    *first = sc.first;
     return sp;
 }
 
-// Walks the segments of a range.
+// Walks the segments of a range: pages p0 .. p1 - 1 (at least one) of item
+// (s, h).
 struct Walk {
     Seq q;
-    int s, h;         // item
-    int p0, p1;       // its pages in this range
-    long long u, end;
-    __device__ bool start(const Args& a, int s_, long long first, long long from, long long to) {
-        s = s_;
-        u = from;
+    int s, h, p0, p1;
+    int item, end;  // the item's first unit; the end of the range
+    __device__ bool start(const Args& a, const Found& f, int from, int to) {
+        s = f.s;
         end = to;
-        if (u >= end || s >= a.seqs) return false;
-        q = seq_of(a, s);
-        h = (int)((u - first) / q.np);
-        p0 = (int)((u - first) - (long long)h * q.np);
-        p1 = (int)min((long long)q.np, p0 + (end - u));
-        return true;
+        if (from >= end || s >= a.seqs) return false;
+        q = f.q;
+        h = (from - f.first) / (q.np + SEG);
+        item = f.first + h * (q.np + SEG);
+        p0 = max(0, from - item - SEG);
+        p1 = min(q.np, end - item - SEG);
+        return p1 > p0 || next(a);
     }
     __device__ bool next(const Args& a) {
-        u += p1 - p0;
-        if (u >= end) return false;
+        item += q.np + SEG;
+        if (item + SEG >= end) return false;  // no page of the next item
         if (++h >= a.kv_heads) {
             h = 0;
             do {
@@ -170,8 +187,15 @@ struct Walk {
             } while (q.np == 0);
         }
         p0 = 0;
-        p1 = (int)min((long long)q.np, end - u);
+        p1 = min(q.np, end - item - SEG);
         return true;
+    }
+    // Worker w's entry of ws_join, (row of node 0, nodes, KV head, partials), from
+    // its first segment (`work`: it has one).
+    __device__ int4 join(const Split& sp, int w, bool work) const {
+        if (!work || p0 == 0) return make_int4(0, 0, 0, 0);
+        if (sp.at(w - 1) > item + SEG) return make_int4(0, 0, 0, 0);  // an earlier worker says it
+        return make_int4(q.lo, q.n, h, sp.worker_of(item + q.np + SEG - 1) - w + 2);
     }
     __device__ bool whole() const { return p0 == 0 && p1 == q.np; }
     __device__ int slot() const { return p0 > 0 ? 0 : 1; }
@@ -209,6 +233,10 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// i / d for 0 <= i < 2^15, 1 <= d <= 128, inv = 1 / d in f32: (i + 0.5) / d is at
+// least 0.5 / 128 away from a whole number, the rounding below 2^-8.
+__device__ __forceinline__ int div_small(int i, float inv) { return (int)(((float)i + 0.5f) * inv); }
+
 constexpr float LN2 = 0.6931471805599453f;
 
 // Tensor-core kernel (tree_attn_tc.cu): query rows of a tile, CTAs per SM, and
@@ -216,7 +244,7 @@ constexpr float LN2 = 0.6931471805599453f;
 constexpr int TC_CTAS_PER_SM = 2;
 constexpr int tc_tile_rows(bool f32) { return f32 ? 64 : 128; }
 jl_status tc_configure();
-jl_status tc_launch(const Args& a, bool f32, cudaStream_t st);
+jl_status tc_launch(Args a, bool f32, cudaStream_t st);
 
 }  // namespace tree
 }  // namespace jl

@@ -8,7 +8,7 @@
 //   * The softmax thread reads its row's 64 scores, masks those it does not
 //     see (only on pages past the committed positions), and writes the weights
 //     2^(s c2 - m) back over the scores as bf16 pieces (two for bf16 outputs,
-//     which leaves 2^-17, and three for f32): the A operand of the next MMA.
+//     which leaves 2^-16, and three for f32): the A operand of the next MMA.
 //   * O += P V accumulates in TMEM over the whole segment.  m is the maximum
 //     when it was last moved: it moves, and O is rescaled, only when a row's
 //     maximum has grown by more than 2^8, so that pages seldom touch O.
@@ -60,7 +60,7 @@ template <int NK, int NV>
 struct Ctl {
     uint64_t kfull[NK], kempty[NK], vfull[NV], vempty[NV];
     uint64_t sfull[2], pfull[2], odone[2];  // by page parity
-    uint64_t qfull, drain;
+    uint64_t qfull, ofree, drain;
     uint32_t tmem;
     int stop;  // a wait gave up: every role leaves
     LocateScratch locate;
@@ -82,6 +82,26 @@ __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volat
     return false;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<uint64_t&>(d))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t&>(d))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+    return d;
+}
+
 __device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -90,24 +110,27 @@ __device__ __forceinline__ float lo_f(uint32_t w) { return __uint_as_float(w << 
 __device__ __forceinline__ float hi_f(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
 // Query rows of a tile into shared memory as bf16 pieces, by the 128 softmax
-// threads: [piece][64-dim block][row][128 B], swizzled.
-__device__ __forceinline__ void load_q(const Args& a, const Walk& w, int row0, int live, uint8_t* sm, int tid, const uint16_t*) {
+// threads: [piece][64-dim block][row][128 B], swizzled.  bf16 rows of groups
+// that divide the tile come by TMA instead.
+__device__ __forceinline__ void load_q(const Args& a, const Walk& w, int row0, int live, float inv_group, uint8_t* sm, int tid,
+                                       const uint16_t*) {
     constexpr int R = Cfg<uint16_t>::ROWS;
-#pragma unroll 4
+    const uint16_t* q = (const uint16_t*)a.q + (size_t)w.q.lo * a.q_ld + (size_t)w.h * a.group * HEAD;
+#pragma unroll 8
     for (int i = tid; i < live * 16; i += 128) {
-        const int r = i >> 4, c = i & 15, g = row0 + r;
-        const uint4 v = *(const uint4*)((const uint16_t*)a.q + (size_t)(w.q.lo + g / a.group) * a.q_ld +
-                                        (size_t)(w.h * a.group + g % a.group) * HEAD + 8 * c);
+        const int r = i >> 4, c = i & 15, node = div_small(row0 + r, inv_group), h = row0 + r - node * a.group;
+        const uint4 v = *(const uint4*)(q + node * a.q_ld + h * HEAD + 8 * c);
         *(uint4*)(sm + (c >> 3) * (R * 128) + swz128((uint32_t)r, (uint32_t)(c & 7) * 16)) = v;
     }
 }
-__device__ __forceinline__ void load_q(const Args& a, const Walk& w, int row0, int live, uint8_t* sm, int tid, const float*) {
+__device__ __forceinline__ void load_q(const Args& a, const Walk& w, int row0, int live, float inv_group, uint8_t* sm, int tid,
+                                       const float*) {
     constexpr int R = Cfg<float>::ROWS;
-#pragma unroll 4
+    const float* q = (const float*)a.q + (size_t)w.q.lo * a.q_ld + (size_t)w.h * a.group * HEAD;
+#pragma unroll 8
     for (int i = tid; i < live * 32; i += 128) {
-        const int r = i >> 5, c = i & 31, g = row0 + r;
-        float4 v = *(const float4*)((const float*)a.q + (size_t)(w.q.lo + g / a.group) * a.q_ld +
-                                    (size_t)(w.h * a.group + g % a.group) * HEAD + 4 * c);
+        const int r = i >> 5, c = i & 31, node = div_small(row0 + r, inv_group), h = row0 + r - node * a.group;
+        float4 v = *(const float4*)(q + node * a.q_ld + h * HEAD + 4 * c);
         uint8_t* dst = sm + (c >> 4) * (R * 128) + swz128((uint32_t)r, (uint32_t)(c & 15) * 8);
 #pragma unroll
         for (int p = 0; p < 3; ++p) {
@@ -118,7 +141,15 @@ __device__ __forceinline__ void load_q(const Args& a, const Walk& w, int row0, i
     }
 }
 
-// S = Q K^T of one page, pieces smallest first.
+// Shared-memory matrix descriptors of 128-byte-swizzled operands (ptx::smem_desc
+// with a stride of 1024 bytes).  Only the low word depends on the address, so
+// the issuing thread adds constants to it: building each descriptor from its
+// address costs more than the MMA takes.
+constexpr uint32_t DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo) { return (saddr >> 4) | ((lbo >> 4) << 16); }
+__device__ __forceinline__ uint64_t desc(uint32_t lo) { return (uint64_t)DESC_HI << 32 | lo; }
+
+// S = Q K^T of one page, pieces smallest first; q, k: low words.
 template <typename T>
 __device__ __forceinline__ void issue_scores(uint32_t q, uint32_t k, uint32_t tmem_s) {
     constexpr uint32_t blk = Cfg<T>::ROWS * 128;
@@ -129,9 +160,8 @@ __device__ __forceinline__ void issue_scores(uint32_t q, uint32_t k, uint32_t tm
         for (int db = 0; db < 2; ++db)
 #pragma unroll
             for (int s = 0; s < 4; ++s)
-                ptx::mma_bf16(tmem_s, ptx::smem_desc(q + (2 * p + db) * blk + 32 * s, 16, 1024, 2),
-                              ptx::smem_desc(k + db * BOX_BYTES + 32 * s, 16, 1024, 2), idesc,
-                              (p < Cfg<T>::NQ - 1 || db || s) ? 1u : 0u);
+                ptx::mma_bf16(tmem_s, desc(q + (((2 * p + db) * blk + 32 * s) >> 4)), desc(k + ((db * BOX_BYTES + 32 * s) >> 4)),
+                              idesc, (p < Cfg<T>::NQ - 1 || db || s) ? 1u : 0u);
 }
 
 // Columns of piece p of the weights.  Two pieces: over the buffer's scores.
@@ -142,8 +172,8 @@ __device__ __forceinline__ uint32_t piece_col(int p) {
     return p < 2 ? 64u + 32u * p : 0u;
 }
 
-// O += P V of one page: P from TMEM, V as an MN-major operand (64-dim blocks
-// BOX_BYTES apart, groups of 8 keys 1024 bytes apart).
+// O += P V of one page: P from TMEM, V (low word v) as an MN-major operand
+// (64-dim blocks BOX_BYTES apart, groups of 8 keys 1024 bytes apart).
 template <typename T>
 __device__ __forceinline__ void issue_pv(uint32_t tmem_p, uint32_t v, uint32_t tmem_o, bool first) {
     const uint32_t idesc = ptx::bf16_idesc(128, HEAD) | (1u << 16);
@@ -151,8 +181,8 @@ __device__ __forceinline__ void issue_pv(uint32_t tmem_p, uint32_t v, uint32_t t
     for (int p = Cfg<T>::NP - 1; p >= 0; --p)
 #pragma unroll
         for (int s = 0; s < 4; ++s)  // keys 16 s ..
-            ptx::mma_bf16_ta(tmem_o, tmem_p + piece_col<T>(p) + 8 * s, ptx::smem_desc(v + 2048 * s, BOX_BYTES, 1024, 2),
-                             idesc, (p < Cfg<T>::NP - 1 || s || !first) ? 1u : 0u);
+            ptx::mma_bf16_ta(tmem_o, tmem_p + piece_col<T>(p) + 8 * s, desc(v + (2048 * s >> 4)), idesc,
+                             (p < Cfg<T>::NP - 1 || s || !first) ? 1u : 0u);
 }
 
 __device__ __forceinline__ bool odd_bf16(uint32_t h) { return (h & 0x7f80u) == 0x7f80u; }  // infinite or NaN
@@ -264,7 +294,8 @@ __device__ __forceinline__ void store_row32<uint16_t>(uint16_t* dst, const float
 
 template <typename T>
 __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
-    k_tree_attn_tc(Args a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+    k_tree_attn_tc(Args a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                   const __grid_constant__ CUtensorMap qmap) {
     constexpr int ROWS = Cfg<T>::ROWS, SB = Cfg<T>::SB, NK = Cfg<T>::NK, NV = Cfg<T>::NV, NP = Cfg<T>::NP;
     extern __shared__ __align__(1024) uint8_t sm[];
     uint8_t* kring = sm + q_bytes<T>();
@@ -287,12 +318,14 @@ __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
             ptx::mbar_init(&ctl.pfull[i], 4);
             ptx::mbar_init(&ctl.odone[i], 1);
         }
-        ptx::mbar_init(&ctl.qfull, 4);
+        ptx::mbar_init(&ctl.qfull, a.q_tma ? 1 : 4);
+        ptx::mbar_init(&ctl.ofree, 4);
         ptx::mbar_init(&ctl.drain, 1);
         ptx::fence_barrier_init();
         ctl.stop = 0;
         ptx::prefetch_tensormap(&kmap);
         ptx::prefetch_tensormap(&vmap);
+        if (a.q_tma) ptx::prefetch_tensormap(&qmap);
     }
     if (warp == W_MMA) {
         ptx::tmem_alloc(&ctl.tmem, TMEM_COLS);
@@ -304,20 +337,26 @@ __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
     const uint32_t tmem = ctl.tmem;
     ptx::grid_dependency_wait();
     ptx::launch_dependents();
-    int s;
-    long long first;
-    const Split sp = locate<T_THREADS>(a, worker, ctl.locate, &s, &first);
+    const Split sp = locate<T_THREADS>(a, worker, ctl.locate);
     Walk w;
-    const bool work = worker < sp.used && w.start(a, s, first, sp.at(worker), sp.at(worker + 1)) &&
-                      !(ptx::smem_u32(sm) & 1023);
+    const bool work = w.start(a, ctl.locate.found, sp.at(worker), sp.at(worker + 1)) && !(ptx::smem_u32(sm) & 1023);
     const int row0 = tile * ROWS;
+    if (tid == 0 && tile == 0 && a.workers > 1) a.ws_join[worker] = w.join(sp, worker, work);
 
     if (work && warp == W_TMA && lane == 0) {
         const int none = a.pages * a.kv_heads * PAGE;  // the row after the pool's last
-        uint32_t it = 0;
+        uint32_t it = 0, seg = 0;
         bool ok = true;
+        auto queries = [&]() {
+            const int node = row0 / a.group;
+            ptx::mbar_arrive_expect_tx(&ctl.qfull, ROWS * HEAD * 2);
+            ptx::tma_load_3d(sm, &qmap, 0, w.h * a.group, w.q.lo + node, &ctl.qfull);
+            ptx::tma_load_3d(sm + ROWS * 128, &qmap, 64, w.h * a.group, w.q.lo + node, &ctl.qfull);
+            ++seg;
+        };
         do {
             if (w.q.n * a.group <= row0) continue;
+            if (a.q_tma && it == 0) queries();
             const int32_t* pt = a.page_table + (size_t)w.s * a.max_pages;
             for (int p = w.p0; ok && p < w.p1; ++p, ++it) {
                 const int page = pt[p];
@@ -340,45 +379,56 @@ __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
                     ptx::tma_load_2d(vring + vs * PAGE_BYTES, &vmap, 0, y, &ctl.vfull[vs]);
                     ptx::tma_load_2d(vring + vs * PAGE_BYTES + BOX_BYTES, &vmap, 64, y, &ctl.vfull[vs]);
                 }
+                if (ok && a.q_tma && p == w.p0 && it > 0) {  // once the last segment's scores are done
+                    const uint32_t j = it - 1;
+                    ok = wait_phase(&ctl.kempty[j % NK], (j / NK) & 1, stop);
+                    if (ok) queries();
+                }
             }
         } while (ok && w.next(a));
         // every copy in flight lands before the shared memory is given up
         for (uint32_t i = it > NK ? it - NK : 0; i < it; ++i) ptx::mbar_wait(&ctl.kfull[i % NK], (i / NK) & 1, WAIT_POLLS);
         for (uint32_t i = it > NV ? it - NV : 0; i < it; ++i) ptx::mbar_wait(&ctl.vfull[i % NV], (i / NV) & 1, WAIT_POLLS);
+        if (seg > 0) ptx::mbar_wait(&ctl.qfull, (seg - 1) & 1, WAIT_POLLS);
     } else if (work && warp == W_MMA && lane == 0) {
-        const uint32_t q = ptx::smem_u32(sm), kr = ptx::smem_u32(kring), vr = ptx::smem_u32(vring);
+        const uint32_t q = desc_lo(ptx::smem_u32(sm), 16), kr = desc_lo(ptx::smem_u32(kring), 16);
+        const uint32_t vr = desc_lo(ptx::smem_u32(vring), BOX_BYTES);
         uint32_t it = 0, seg = 0;
         bool ok = true;
         auto scores = [&](uint32_t i) {
             ok = wait_phase(&ctl.kfull[i % NK], (i / NK) & 1, stop);
             if (!ok) return;
             ptx::tc_fence_after();
-            issue_scores<T>(q, kr + (i % NK) * PAGE_BYTES, tmem + 64 * (i % SB));
+            issue_scores<T>(q, kr + (i % NK) * (PAGE_BYTES >> 4), tmem + 64 * (i % SB));
             ptx::tc_commit(&ctl.kempty[i % NK]);
             ptx::tc_commit(&ctl.sfull[i & 1]);
         };
         do {
             if (w.q.n * a.group <= row0) continue;
             const int n = w.p1 - w.p0;
-            ok = wait_phase(&ctl.qfull, seg++ & 1, stop);
+            ok = wait_phase(&ctl.qfull, seg & 1, stop);
             if (ok) scores(it);
             for (int i = 0; ok && i < n; ++i, ++it) {
                 if (SB == 2 && i + 1 < n) scores(it + 1);
                 ok = ok && wait_phase(&ctl.pfull[it & 1], (it >> 1) & 1, stop) &&
                      wait_phase(&ctl.vfull[it % NV], (it / NV) & 1, stop);
+                // the last segment's O was read
+                if (i == 0 && seg > 0) ok = ok && wait_phase(&ctl.ofree, (seg - 1) & 1, stop);
                 if (!ok) break;
                 ptx::tc_fence_after();
-                issue_pv<T>(tmem + 64 * (it % SB), vr + (it % NV) * PAGE_BYTES, tmem + COL_O, i == 0);
+                issue_pv<T>(tmem + 64 * (it % SB), vr + (it % NV) * (PAGE_BYTES >> 4), tmem + COL_O, i == 0);
                 ptx::tc_commit(&ctl.vempty[it % NV]);
                 ptx::tc_commit(&ctl.odone[it & 1]);
                 if (SB == 1 && i + 1 < n) scores(it + 1);
             }
+            ++seg;
         } while (ok && w.next(a));
         // every MMA is done before TMEM and the shared memory are given up
         ptx::tc_commit(&ctl.drain);
         ptx::mbar_wait(&ctl.drain, 0, WAIT_POLLS);
     } else if (work && warp < 4) {
         const uint32_t t_lane = tmem + ((uint32_t)(warp * 32) << 16);
+        const float inv_group = 1.f / a.group;
         uint32_t it = 0;
         bool ok = true;
         do {
@@ -386,25 +436,27 @@ __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
             if (live <= 0) continue;
             const int g = row0 + tid, n = w.p1 - w.p0;
             const bool mine = tid < live, active = warp * 32 < live;
-            load_q(a, w, row0, live, sm, tid, (const T*)nullptr);
-            ptx::fence_proxy_async_smem();
-            ptx::tc_fence_before();  // and the last segment's reads of O are done
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(&ctl.qfull);
+            const int node = div_small(g, inv_group), head = w.h * a.group + g - node * a.group;
+            if (!a.q_tma) {
+                load_q(a, w, row0, live, inv_group, sm, tid, (const T*)nullptr);
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(&ctl.qfull);
+            }
             const int32_t* pt = a.page_table + (size_t)w.s * a.max_pages;
             float m = -INFINITY, l = 0.f;
             bool odd = false;  // this thread took a value out
+            int page = pt[w.p0];
             for (int i = 0; ok && i < n; ++i, ++it) {
                 const int p = w.p0 + i;
-                const int page = pt[p];
                 const bool there = (unsigned)page < (unsigned)a.pages;
-                const bool edge = !there || (long long)(p + 1) * PAGE > w.q.ctx;
+                const bool edge = !there || (p + 1) * PAGE > w.q.ctx;
+                if (i + 1 < n) page = pt[p + 1];
                 if (edge) {
                     ok = wait_phase(&ctl.vfull[it % NV], (it / NV) & 1, stop);
                     if (ok) {
-                        const long long left = (long long)w.q.ctx + w.q.n - (long long)p * PAGE;
-                        odd |= clean_v(vring + (it % NV) * PAGE_BYTES, max(0, (int)min(64ll, w.q.ctx - (long long)p * PAGE)),
-                                       there ? (int)min(64ll, left) : 0, tid);
+                        odd |= clean_v(vring + (it % NV) * PAGE_BYTES, max(0, w.q.ctx - p * PAGE),
+                                       there ? w.q.ctx + w.q.n - p * PAGE : 0, tid);
                         ptx::fence_proxy_async_smem();
                     }
                 }
@@ -417,7 +469,7 @@ __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
                     float x[64];
                     ptx::tmem_ld64_sync(t_s, x);
                     if (edge) {
-                        const uint64_t vis = mine && there ? visible(a, w.q, g / a.group, p) : 0;
+                        const uint64_t vis = mine && there ? visible(a, w.q, node, p) : 0;
                         const uint32_t v0 = (uint32_t)vis, v1 = (uint32_t)(vis >> 32);
 #pragma unroll
                         for (int c = 0; c < 32; ++c) {
@@ -425,13 +477,19 @@ __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
                             if (!(v1 >> c & 1)) x[32 + c] = -INFINITY;
                         }
                     }
-                    float t0 = fmaxf(x[0], x[1]), t1 = fmaxf(x[2], x[3]);
+                    float t0 = max3(x[0], x[1], x[2]), t1 = max3(x[3], x[4], x[5]);
+                    float t2 = max3(x[6], x[7], x[8]), t3 = max3(x[9], x[10], x[11]);
 #pragma unroll
-                    for (int c = 4; c < 64; c += 4) {
-                        t0 = fmaxf(t0, fmaxf(x[c], x[c + 1]));
-                        t1 = fmaxf(t1, fmaxf(x[c + 2], x[c + 3]));
+                    for (int c = 12; c < 60; c += 8) {
+                        t0 = max3(t0, x[c], x[c + 1]);
+                        t1 = max3(t1, x[c + 2], x[c + 3]);
+                        t2 = max3(t2, x[c + 4], x[c + 5]);
+                        t3 = max3(t3, x[c + 6], x[c + 7]);
                     }
-                    const float top = fmaxf(t0, t1) * a.c2;
+                    t0 = max3(t0, x[60], x[61]);
+                    t1 = max3(t1, x[62], x[63]);
+                    t0 = max3(t0, t1, t2);
+                    const float top = fmaxf(t0, t3) * a.c2;
                     float f = 1.f;
                     if (m == -INFINITY) {
                         m = top;  // nothing was seen before: O and l are zero
@@ -456,24 +514,32 @@ __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
                         }
                     }
                     const float ref = m == -INFINITY ? 0.f : m;
-                    float s0 = 0.f, s1 = 0.f;
+                    const float2 c2 = make_float2(a.c2, a.c2), nref = make_float2(-ref, -ref);
+                    float2 s0 = make_float2(0.f, 0.f), s1 = s0;
 #pragma unroll
-                    for (int c = 0; c < 64; c += 2) {
-                        x[c] = ex2(fmaf(x[c], a.c2, -ref));
-                        x[c + 1] = ex2(fmaf(x[c + 1], a.c2, -ref));
-                        s0 += x[c];
-                        s1 += x[c + 1];
+                    for (int c = 0; c < 64; c += 4) {
+                        float2 y = fma2(make_float2(x[c], x[c + 1]), c2, nref);
+                        float2 z = fma2(make_float2(x[c + 2], x[c + 3]), c2, nref);
+                        y = make_float2(ex2(y.x), ex2(y.y));
+                        z = make_float2(ex2(z.x), ex2(z.y));
+                        s0 = add2(s0, y);
+                        s1 = add2(s1, z);
+                        x[c] = y.x, x[c + 1] = y.y, x[c + 2] = z.x, x[c + 3] = z.y;
                     }
-                    l += s0 + s1;
+                    s0 = add2(s0, s1);
+                    l += s0.x + s0.y;
+                    // pieces by truncation: each takes the next 8 bits, exactly
 #pragma unroll
                     for (int pc = 0; pc < NP; ++pc) {
                         uint32_t r[32];
 #pragma unroll
                         for (int c = 0; c < 32; ++c) {
-                            r[c] = pack_bf16(x[2 * c], x[2 * c + 1]);
+                            const uint32_t u = __float_as_uint(x[2 * c]), v = __float_as_uint(x[2 * c + 1]);
+                            r[c] = __byte_perm(u, v, 0x7632);
                             if (pc + 1 < NP) {
-                                x[2 * c] -= lo_f(r[c]);
-                                x[2 * c + 1] -= hi_f(r[c]);
+                                const float2 d = add2(make_float2(x[2 * c], x[2 * c + 1]),
+                                                      make_float2(-__uint_as_float(u & 0xffff0000u), -__uint_as_float(v & 0xffff0000u)));
+                                x[2 * c] = d.x, x[2 * c + 1] = d.y;
                             }
                         }
                         ptx::tmem_st32(t_s + piece_col<T>(pc), r);
@@ -497,7 +563,7 @@ __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
                 const bool whole = w.whole();
                 const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);  // 0: nothing seen
                 const size_t part = (((size_t)worker * a.lanes + tile) * 2 + w.slot()) * ROWS + tid;
-                const int row = w.q.lo + g / a.group, head = w.h * a.group + g % a.group;
+                const int row = w.q.lo + node;
 #pragma unroll 1
                 for (int c = 0; c < HEAD; c += 32) {
                     float o[32];
@@ -510,8 +576,12 @@ __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
                 if (mine && whole && a.lse) a.lse[(size_t)row * a.q_heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
                 if (mine && !whole) *(float2*)(a.ws_ml + part * 2) = make_float2(m, l);
             }
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&ctl.ofree);
         } while (w.next(a));
     }
+
     __syncwarp();
     __syncthreads();
     if (tid == 0 && (ctl.stop || (ptx::smem_u32(sm) & 1023))) flag(a.status, ST_TIMEOUT);
@@ -520,8 +590,8 @@ __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
 }
 
 template <typename T>
-jl_status launch(const Args& a, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st) {
-    return launch_pdl(k_tree_attn_tc<T>, dim3(a.workers, a.lanes), dim3(T_THREADS), tc_smem<T>(), st, a, k, v);
+jl_status launch(const Args& a, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& q, cudaStream_t st) {
+    return launch_pdl(k_tree_attn_tc<T>, dim3(a.workers, a.lanes), dim3(T_THREADS), tc_smem<T>(), st, a, k, v, q);
 }
 
 }  // namespace
@@ -533,12 +603,15 @@ jl_status tc_configure() {
     return JL_OK;
 }
 
-jl_status tc_launch(const Args& a, bool f32, cudaStream_t st) {
+jl_status tc_launch(Args a, bool f32, cudaStream_t st) {
     const uint64_t rows = (uint64_t)a.pages * a.kv_heads * PAGE;
-    CUtensorMap k, v;
+    CUtensorMap k, v, q{};
     JL_TRY(kv_page_map(&k, const_cast<void*>(a.k), rows));
     JL_TRY(kv_page_map(&v, const_cast<void*>(a.v), rows));
-    return f32 ? launch<float>(a, k, v, st) : launch<uint16_t>(a, k, v, st);
+    // bf16 queries by TMA: rows (node, head of the group) of a tile are one box
+    a.q_tma = !f32 && tc_tile_rows(false) % a.group == 0;
+    if (a.q_tma) JL_TRY(q_row_map(&q, a.q, a.q_heads, a.rows, a.q_ld, a.group, tc_tile_rows(false) / a.group));
+    return f32 ? launch<float>(a, k, v, q, st) : launch<uint16_t>(a, k, v, q, st);
 }
 
 }  // namespace tree
