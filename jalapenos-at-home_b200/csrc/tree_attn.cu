@@ -360,7 +360,7 @@ Plan plan_of(const jl_tree_attn& a, int sms) {
     p.tile_rows = tc ? tc_tile_rows(a.dtype == JL_KV_F32) : rows <= 16 ? 16 : 64;
     p.lanes = (rows + p.tile_rows - 1) / p.tile_rows;
     p.workers = std::min(CB_MOST, std::max(1, (tc ? TC_CTAS_PER_SM : 1) * sms / p.lanes));
-    p.min_units = 4 + SEG;  // four pages and a start
+    p.min_units = 1 + SEG;
     p.bytes = p.workers == 1 ? 0 : (size_t)p.workers * (sizeof(int4) + (size_t)p.lanes * 2 * p.tile_rows * (HEAD + 2) * sizeof(float));
     return p;
 }

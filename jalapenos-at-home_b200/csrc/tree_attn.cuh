@@ -242,7 +242,7 @@ constexpr float LN2 = 0.6931471805599453f;
 // Tensor-core kernel (tree_attn_tc.cu): query rows of a tile, CTAs per SM, and
 // the launch over a pool of bf16 pages; `f32`: the type of the q and out rows.
 constexpr int TC_CTAS_PER_SM = 2;
-constexpr int tc_tile_rows(bool f32) { return f32 ? 64 : 128; }
+constexpr int tc_tile_rows(bool f32) { return f32 ? 32 : 128; }
 jl_status tc_configure();
 jl_status tc_launch(Args a, bool f32, cudaStream_t st);
 

@@ -3,18 +3,23 @@
 // A CTA walks its worker's range (tree_attn.cuh) page by page with six warps:
 // warp 5 brings K and V pages into two rings by TMA, warp 4 issues the MMAs,
 // and warps 0-3 do the softmax, a thread per query row (MMA row = TMEM lane).
-//   * S = Q K^T (128 x 64 f32) goes to TMEM.  Queries are exact in bf16; f32
-//     queries enter as three bf16 pieces (24 bits), smallest first.
+//   * S = Q K^T (128 x 64 f32) goes to TMEM.  bf16 queries are exact.
 //   * The softmax thread reads its row's 64 scores, masks those it does not
 //     see (only on pages past the committed positions), and writes the weights
-//     2^(s c2 - m) back over the scores as bf16 pieces (two for bf16 outputs,
-//     which leaves 2^-16, and three for f32): the A operand of the next MMA.
+//     2^(s c2 - m) back over the scores as bf16 pieces, the A operand of the
+//     next MMA: two for bf16 outputs, which leaves 2^-16.
 //   * O += P V accumulates in TMEM over the whole segment.  m is the maximum
 //     when it was last moved: it moves, and O is rescaled, only when a row's
 //     maximum has grown by more than 2^8, so that pages seldom touch O.
-//   * With bf16 rows the scores of page j + 1 are computed while page j's
-//     weights are (two S buffers).  Three pieces fill that space, so f32 rows
-//     take one buffer and leave the overlap to the second CTA of the SM.
+//   * The scores of page j + 1 are computed while page j's weights are (two S
+//     buffers).
+// f32 rows are stacked: a tile has 32 rows, and lanes 32 p + r hold piece p of
+// row r's three bf16 pieces (24 bits), so that one MMA of 128 rows multiplies
+// all pieces.  Warps 0-2 exchange their parts of S through shared memory, all
+// compute the same weights, and warp p writes the weights' piece p; the three
+// parts of O are added at the end.  Against three MMAs a product with all pieces
+// in the rows of one tile of 64, a page takes a third of the MMA time (16
+// sequences of 8 nodes and 4 heads a KV head at 2000 positions: MEASURED).
 // Sums, maxima and O are f32.  V rows past the sequence, and values of tree
 // nodes that are not finite, are cleared in shared memory before P V (zero
 // times them would be NaN in rows that do not see them); rows that do see such
@@ -44,17 +49,20 @@ constexpr uint32_t COL_O = 128, TMEM_COLS = 256;
 constexpr uint32_t WAIT_POLLS = 1u << 20;
 constexpr float MOVE = 8.f;  // log2 of how far a row's maximum may grow before it is moved
 
+// NP: pieces of the weights in a row's columns.  SPLIT: warps that hold the
+// pieces of the same rows.
 template <typename T>
 struct Cfg;
 template <>
 struct Cfg<uint16_t> {
-    static constexpr int ROWS = tc_tile_rows(false), NQ = 1, NP = 2, SB = 2, NK = 3, NV = 2;
+    static constexpr int ROWS = tc_tile_rows(false), NP = 2, SPLIT = 1, NK = 3, NV = 2, Q_ROWS = 128, XCH = 0;
 };
 template <>
 struct Cfg<float> {
-    // 64 rows: three pieces of them take 48 KB, which leaves two CTAs an SM
-    static constexpr int ROWS = tc_tile_rows(true), NQ = 3, NP = 3, SB = 1, NK = 2, NV = 2;
+    static constexpr int ROWS = tc_tile_rows(true), NP = 1, SPLIT = 3, NK = 2, NV = 2, Q_ROWS = SPLIT * ROWS;
+    static constexpr int XCH = SPLIT * ROWS * 64 * 4;  // the exchange: 64 floats of every row and part
 };
+constexpr int SB = 2;  // S buffers
 
 template <int NK, int NV>
 struct Ctl {
@@ -67,9 +75,10 @@ struct Ctl {
 };
 
 template <typename T>
-constexpr uint32_t q_bytes() { return Cfg<T>::NQ * Cfg<T>::ROWS * HEAD * 2; }
+constexpr uint32_t q_bytes() { return Cfg<T>::Q_ROWS * HEAD * 2; }
 template <typename T>
-constexpr size_t tc_smem() { return q_bytes<T>() + (size_t)(Cfg<T>::NK + Cfg<T>::NV) * PAGE_BYTES + 1024; }
+constexpr size_t tc_smem() { return q_bytes<T>() + (size_t)(Cfg<T>::NK + Cfg<T>::NV) * PAGE_BYTES + Cfg<T>::XCH + 1024; }
+static_assert(tc_smem<float>() <= 113 * 1024 && tc_smem<uint16_t>() <= 113 * 1024, "two CTAs an SM");
 static_assert(sizeof(Ctl<3, 2>) <= 1024, "control block");
 
 // Waits for a phase, for WAIT_POLLS polls or until another role stops.
@@ -110,8 +119,8 @@ __device__ __forceinline__ float lo_f(uint32_t w) { return __uint_as_float(w << 
 __device__ __forceinline__ float hi_f(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
 // Query rows of a tile into shared memory as bf16 pieces, by the 128 softmax
-// threads: [piece][64-dim block][row][128 B], swizzled.  bf16 rows of groups
-// that divide the tile come by TMA instead.
+// threads: [64-dim block][lane][128 B], swizzled.  bf16 rows of groups that
+// divide the tile come by TMA instead.
 __device__ __forceinline__ void load_q(const Args& a, const Walk& w, int row0, int live, float inv_group, uint8_t* sm, int tid,
                                        const uint16_t*) {
     constexpr int R = Cfg<uint16_t>::ROWS;
@@ -125,17 +134,18 @@ __device__ __forceinline__ void load_q(const Args& a, const Walk& w, int row0, i
 }
 __device__ __forceinline__ void load_q(const Args& a, const Walk& w, int row0, int live, float inv_group, uint8_t* sm, int tid,
                                        const float*) {
-    constexpr int R = Cfg<float>::ROWS;
+    constexpr int R = Cfg<float>::ROWS, Q = Cfg<float>::Q_ROWS;
     const float* q = (const float*)a.q + (size_t)w.q.lo * a.q_ld + (size_t)w.h * a.group * HEAD;
-#pragma unroll 8
-    for (int i = tid; i < live * 32; i += 128) {
-        const int r = i >> 5, c = i & 31, node = div_small(row0 + r, inv_group), h = row0 + r - node * a.group;
-        float4 v = *(const float4*)(q + node * a.q_ld + h * HEAD + 4 * c);
-        uint8_t* dst = sm + (c >> 4) * (R * 128) + swz128((uint32_t)r, (uint32_t)(c & 15) * 8);
 #pragma unroll
-        for (int p = 0; p < 3; ++p) {
+    for (int i = tid; i < R * 32; i += 128) {
+        const int r = i >> 5, c = i & 31;
+        if (r >= live) break;
+        const int node = div_small(row0 + r, inv_group), h = row0 + r - node * a.group;
+        float4 v = *(const float4*)(q + node * a.q_ld + h * HEAD + 4 * c);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {  // lanes 32 p + r
             const uint32_t x = pack_bf16(v.x, v.y), y = pack_bf16(v.z, v.w);
-            *(uint2*)(dst + p * (2 * R * 128)) = make_uint2(x, y);
+            *(uint2*)(sm + (c >> 4) * (Q * 128) + swz128((uint32_t)(p * R + r), (uint32_t)(c & 15) * 8)) = make_uint2(x, y);
             v = make_float4(v.x - lo_f(x), v.y - hi_f(x), v.z - lo_f(y), v.w - hi_f(y));
         }
     }
@@ -149,27 +159,27 @@ constexpr uint32_t DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
 __device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo) { return (saddr >> 4) | ((lbo >> 4) << 16); }
 __device__ __forceinline__ uint64_t desc(uint32_t lo) { return (uint64_t)DESC_HI << 32 | lo; }
 
-// S = Q K^T of one page, pieces smallest first; q, k: low words.
+// S = Q K^T of one page; q, k: low words.
 template <typename T>
 __device__ __forceinline__ void issue_scores(uint32_t q, uint32_t k, uint32_t tmem_s) {
-    constexpr uint32_t blk = Cfg<T>::ROWS * 128;
     const uint32_t idesc = ptx::bf16_idesc(128, PAGE);
 #pragma unroll
-    for (int p = Cfg<T>::NQ - 1; p >= 0; --p)
+    for (int db = 0; db < 2; ++db)
 #pragma unroll
-        for (int db = 0; db < 2; ++db)
-#pragma unroll
-            for (int s = 0; s < 4; ++s)
-                ptx::mma_bf16(tmem_s, desc(q + (((2 * p + db) * blk + 32 * s) >> 4)), desc(k + ((db * BOX_BYTES + 32 * s) >> 4)),
-                              idesc, (p < Cfg<T>::NQ - 1 || db || s) ? 1u : 0u);
+        for (int s = 0; s < 4; ++s)
+            ptx::mma_bf16(tmem_s, desc(q + ((db * Cfg<T>::Q_ROWS * 128 + 32 * s) >> 4)), desc(k + ((db * BOX_BYTES + 32 * s) >> 4)),
+                          idesc, (db || s) ? 1u : 0u);
 }
 
-// Columns of piece p of the weights.  Two pieces: over the buffer's scores.
-// Three: behind them, the last over their first half.
-template <typename T>
-__device__ __forceinline__ uint32_t piece_col(int p) {
-    if (Cfg<T>::NP == 2) return 32u * p;
-    return p < 2 ? 64u + 32u * p : 0u;
+// The exchange between the warps that hold the pieces of 32 f32 rows: floats
+// c .. c + 3 (c a multiple of 4 below 64) of a row's part, swizzled so that eight
+// rows' float4s lie on all banks; and the sum of a row's three parts.
+__device__ __forceinline__ float4* xch_at(uint8_t* xch, int part, int row, int c) {
+    return (float4*)(xch + (part * 32 + row) * 256 + (((c >> 2) ^ (row & 7)) << 4));
+}
+__device__ __forceinline__ float4 xch_sum(uint8_t* xch, int row, int c) {
+    const float4 u = *xch_at(xch, 0, row, c), v = *xch_at(xch, 1, row, c), y = *xch_at(xch, 2, row, c);
+    return make_float4(u.x + (v.x + y.x), u.y + (v.y + y.y), u.z + (v.z + y.z), u.w + (v.w + y.w));
 }
 
 // O += P V of one page: P from TMEM, V (low word v) as an MN-major operand
@@ -181,7 +191,7 @@ __device__ __forceinline__ void issue_pv(uint32_t tmem_p, uint32_t v, uint32_t t
     for (int p = Cfg<T>::NP - 1; p >= 0; --p)
 #pragma unroll
         for (int s = 0; s < 4; ++s)  // keys 16 s ..
-            ptx::mma_bf16_ta(tmem_o, tmem_p + piece_col<T>(p) + 8 * s, desc(v + (2048 * s >> 4)), idesc,
+            ptx::mma_bf16_ta(tmem_o, tmem_p + 32 * p + 8 * s, desc(v + (2048 * s >> 4)), idesc,
                              (p < Cfg<T>::NP - 1 || s || !first) ? 1u : 0u);
 }
 
@@ -262,16 +272,17 @@ __device__ __noinline__ void add_odd(const Args a, const Walk w, int g, bool min
     ptx::tmem_wait_st();
 }
 
-// A barrier of the 128 softmax threads that tells whether `ok` holds for all.
-__device__ __forceinline__ bool all_of_softmax(bool ok) {
+// A barrier of the first N softmax threads that tells whether `ok` holds for all.
+template <int N>
+__device__ __forceinline__ bool all_of(bool ok) {
     uint32_t r;
     asm volatile(
         "{\n .reg .pred p, q;\n"
         " setp.ne.u32 p, %1, 0;\n"
-        " barrier.cta.red.and.pred q, 1, 128, p;\n"
+        " barrier.cta.red.and.pred q, %2, %3, p;\n"
         " selp.u32 %0, 1, 0, q;\n}"
         : "=r"(r)
-        : "r"((uint32_t)ok)
+        : "r"((uint32_t)ok), "n"(N / 32), "n"(N)
         : "memory");
     return r != 0;
 }
@@ -296,11 +307,12 @@ template <typename T>
 __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
     k_tree_attn_tc(Args a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                    const __grid_constant__ CUtensorMap qmap) {
-    constexpr int ROWS = Cfg<T>::ROWS, SB = Cfg<T>::SB, NK = Cfg<T>::NK, NV = Cfg<T>::NV, NP = Cfg<T>::NP;
+    constexpr int ROWS = Cfg<T>::ROWS, NK = Cfg<T>::NK, NV = Cfg<T>::NV, NP = Cfg<T>::NP, SPLIT = Cfg<T>::SPLIT;
     extern __shared__ __align__(1024) uint8_t sm[];
     uint8_t* kring = sm + q_bytes<T>();
     uint8_t* vring = kring + NK * PAGE_BYTES;
-    Ctl<NK, NV>& ctl = *(Ctl<NK, NV>*)(vring + NV * PAGE_BYTES);
+    uint8_t* xch = vring + NV * PAGE_BYTES;
+    Ctl<NK, NV>& ctl = *(Ctl<NK, NV>*)(vring + NV * PAGE_BYTES + Cfg<T>::XCH);
     volatile int* stop = &ctl.stop;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int worker = blockIdx.x, tile = blockIdx.y;
@@ -409,7 +421,7 @@ __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
             ok = wait_phase(&ctl.qfull, seg & 1, stop);
             if (ok) scores(it);
             for (int i = 0; ok && i < n; ++i, ++it) {
-                if (SB == 2 && i + 1 < n) scores(it + 1);
+                if (i + 1 < n) scores(it + 1);
                 ok = ok && wait_phase(&ctl.pfull[it & 1], (it >> 1) & 1, stop) &&
                      wait_phase(&ctl.vfull[it % NV], (it / NV) & 1, stop);
                 // the last segment's O was read
@@ -419,7 +431,6 @@ __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
                 issue_pv<T>(tmem + 64 * (it % SB), vr + (it % NV) * (PAGE_BYTES >> 4), tmem + COL_O, i == 0);
                 ptx::tc_commit(&ctl.vempty[it % NV]);
                 ptx::tc_commit(&ctl.odone[it & 1]);
-                if (SB == 1 && i + 1 < n) scores(it + 1);
             }
             ++seg;
         } while (ok && w.next(a));
@@ -429,13 +440,14 @@ __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
     } else if (work && warp < 4) {
         const uint32_t t_lane = tmem + ((uint32_t)(warp * 32) << 16);
         const float inv_group = 1.f / a.group;
+        const int r = SPLIT > 1 ? lane : tid;  // row of the tile
         uint32_t it = 0;
         bool ok = true;
         do {
             const int live = min(ROWS, w.q.n * a.group - row0);
             if (live <= 0) continue;
-            const int g = row0 + tid, n = w.p1 - w.p0;
-            const bool mine = tid < live, active = warp * 32 < live;
+            const int g = row0 + r, n = w.p1 - w.p0;
+            const bool active = SPLIT > 1 ? warp < SPLIT : warp * 32 < live, mine = active && r < live;
             const int node = div_small(g, inv_group), head = w.h * a.group + g - node * a.group;
             if (!a.q_tma) {
                 load_q(a, w, row0, live, inv_group, sm, tid, (const T*)nullptr);
@@ -447,12 +459,14 @@ __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
             float m = -INFINITY, l = 0.f;
             bool odd = false;  // this thread took a value out
             int page = pt[w.p0];
-            for (int i = 0; ok && i < n; ++i, ++it) {
+            // Warps that exchange leave the loop together: a wait that gives up
+            // only clears ok, until the exchange tells all of them.
+            for (int i = 0; i < n; ++i, ++it) {
                 const int p = w.p0 + i;
                 const bool there = (unsigned)page < (unsigned)a.pages;
                 const bool edge = !there || (p + 1) * PAGE > w.q.ctx;
                 if (i + 1 < n) page = pt[p + 1];
-                if (edge) {
+                if (edge && ok) {
                     ok = wait_phase(&ctl.vfull[it % NV], (it / NV) & 1, stop);
                     if (ok) {
                         odd |= clean_v(vring + (it % NV) * PAGE_BYTES, max(0, w.q.ctx - p * PAGE),
@@ -462,12 +476,26 @@ __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
                 }
                 ok = ok && wait_phase(&ctl.sfull[it & 1], (it >> 1) & 1, stop);
                 ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
+                if (!ok && !(SPLIT > 1 && active)) break;
                 ptx::tc_fence_after();
                 if (active) {
                     const uint32_t t_s = t_lane + 64 * (it % SB);
                     float x[64];
-                    ptx::tmem_ld64_sync(t_s, x);
+                    if (ok) ptx::tmem_ld64_sync(t_s, x);
+                    if constexpr (SPLIT > 1) {  // the pieces' parts of S
+                        if (ok) {
+#pragma unroll
+                            for (int c = 0; c < 64; c += 4) *xch_at(xch, warp, lane, c) = make_float4(x[c], x[c + 1], x[c + 2], x[c + 3]);
+                        }
+                        ok = all_of<32 * SPLIT>(ok);
+                        if (!ok) break;
+#pragma unroll
+                        for (int c = 0; c < 64; c += 4) {
+                            const float4 u = xch_sum(xch, lane, c);
+                            x[c] = u.x, x[c + 1] = u.y, x[c + 2] = u.z, x[c + 3] = u.w;
+                        }
+                        all_of<32 * SPLIT>(true);  // every part was read
+                    }
                     if (edge) {
                         const uint64_t vis = mine && there ? visible(a, w.q, node, p) : 0;
                         const uint32_t v0 = (uint32_t)vis, v1 = (uint32_t)(vis >> 32);
@@ -501,16 +529,15 @@ __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
                     if (i > 0 && __any_sync(0xffffffffu, mine && f != 1.f)) {
                         const uint32_t j = it - 1;  // every earlier P V is done
                         ok = __all_sync(0xffffffffu, wait_phase(&ctl.odone[j & 1], (j >> 1) & 1, stop));
-                        if (!ok) break;
                         ptx::tc_fence_after();
 #pragma unroll 1
-                        for (int c = 0; c < HEAD; c += 32) {
+                        for (int c = 0; ok && c < HEAD; c += 32) {
                             float o[32];
-                            uint32_t r[32];
+                            uint32_t b[32];
                             ptx::tmem_ld32_sync(t_lane + COL_O + c, o);
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(o[e] * f);
-                            ptx::tmem_st32(t_lane + COL_O + c, r);
+                            for (int e = 0; e < 32; ++e) b[e] = __float_as_uint(o[e] * f);
+                            ptx::tmem_st32(t_lane + COL_O + c, b);
                         }
                     }
                     const float ref = m == -INFINITY ? 0.f : m;
@@ -529,20 +556,22 @@ __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
                     s0 = add2(s0, s1);
                     l += s0.x + s0.y;
                     // pieces by truncation: each takes the next 8 bits, exactly
+                    auto rest = [&]() {
+#pragma unroll
+                        for (int c = 0; c < 64; c += 2) {
+                            const float2 d = add2(make_float2(x[c], x[c + 1]), make_float2(-hi_f(__float_as_uint(x[c])), -hi_f(__float_as_uint(x[c + 1]))));
+                            x[c] = d.x, x[c + 1] = d.y;
+                        }
+                    };
+                    for (int k = 0; SPLIT > 1 && k < warp; ++k) rest();
 #pragma unroll
                     for (int pc = 0; pc < NP; ++pc) {
-                        uint32_t r[32];
+                        if (pc) rest();
+                        uint32_t b[32];
 #pragma unroll
-                        for (int c = 0; c < 32; ++c) {
-                            const uint32_t u = __float_as_uint(x[2 * c]), v = __float_as_uint(x[2 * c + 1]);
-                            r[c] = __byte_perm(u, v, 0x7632);
-                            if (pc + 1 < NP) {
-                                const float2 d = add2(make_float2(x[2 * c], x[2 * c + 1]),
-                                                      make_float2(-__uint_as_float(u & 0xffff0000u), -__uint_as_float(v & 0xffff0000u)));
-                                x[2 * c] = d.x, x[2 * c + 1] = d.y;
-                            }
-                        }
-                        ptx::tmem_st32(t_s + piece_col<T>(pc), r);
+                        for (int c = 0; c < 32; ++c)
+                            b[c] = __byte_perm(__float_as_uint(x[2 * c]), __float_as_uint(x[2 * c + 1]), 0x7632);
+                        ptx::tmem_st32(t_s + 32 * pc, b);
                     }
                     ptx::tmem_wait_st();
                 }
@@ -554,34 +583,61 @@ __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
                 const uint32_t j = it - 1;
                 ok = wait_phase(&ctl.odone[j & 1], (j >> 1) & 1, stop);
             }
-            ok = all_of_softmax(ok);
+            ok = all_of<128>(ok);
             if (!ok) break;
             ptx::tc_fence_after();
-            odd = !all_of_softmax(!odd);
+            odd = !all_of<128>(!odd);
             if (active) {
-                if (odd) add_odd<T>(a, w, g, mine, m == -INFINITY ? 0.f : m, t_lane + COL_O);
+                if (odd && (SPLIT == 1 || warp == 0)) add_odd<T>(a, w, g, mine, m == -INFINITY ? 0.f : m, t_lane + COL_O);
                 const bool whole = w.whole();
                 const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);  // 0: nothing seen
-                const size_t part = (((size_t)worker * a.lanes + tile) * 2 + w.slot()) * ROWS + tid;
-                const int row = w.q.lo + node;
+                const size_t part = (((size_t)worker * a.lanes + tile) * 2 + w.slot()) * ROWS + r;
+                T* out = (T*)a.out + (size_t)(w.q.lo + node) * a.out_ld + (size_t)head * HEAD;
+                auto store = [&](int c, const float (&o)[32]) {
+                    if (!mine) return;
+                    if (whole) store_row32<T>(out + c, o, inv);
+                    else store_row32<float>(a.ws_o + part * HEAD + c, o, 1.f);
+                };
+                if constexpr (SPLIT > 1) {  // 64 dims at a time: warp p adds the parts of dims 32 p ..
 #pragma unroll 1
-                for (int c = 0; c < HEAD; c += 32) {
-                    float o[32];
-                    ptx::tmem_ld32_sync(t_lane + COL_O + c, o);
-                    if (mine) {
-                        if (whole) store_row32<T>((T*)a.out + (size_t)row * a.out_ld + (size_t)head * HEAD + c, o, inv);
-                        else store_row32<float>(a.ws_o + part * HEAD + c, o, 1.f);
+                    for (int c = 0; c < HEAD; c += 64) {
+#pragma unroll 1
+                        for (int d = 0; d < 64; d += 32) {
+                            float o[32];
+                            ptx::tmem_ld32_sync(t_lane + COL_O + c + d, o);
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4) *xch_at(xch, warp, lane, d + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                        }
+                        all_of<32 * SPLIT>(true);
+                        if (warp < 2) {
+                            float o[32];
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4) {
+                                const float4 u = xch_sum(xch, lane, 32 * warp + e);
+                                o[e] = u.x, o[e + 1] = u.y, o[e + 2] = u.z, o[e + 3] = u.w;
+                            }
+                            store(c + 32 * warp, o);
+                        }
+                        all_of<32 * SPLIT>(true);
+                    }
+                } else {
+#pragma unroll 1
+                    for (int c = 0; c < HEAD; c += 32) {
+                        float o[32];
+                        ptx::tmem_ld32_sync(t_lane + COL_O + c, o);
+                        store(c, o);
                     }
                 }
-                if (mine && whole && a.lse) a.lse[(size_t)row * a.q_heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
-                if (mine && !whole) *(float2*)(a.ws_ml + part * 2) = make_float2(m, l);
+                if (mine && (SPLIT == 1 || warp == 0)) {
+                    if (!whole) *(float2*)(a.ws_ml + part * 2) = make_float2(m, l);
+                    else if (a.lse) a.lse[(size_t)(w.q.lo + node) * a.q_heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+                }
             }
             ptx::tc_fence_before();
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(&ctl.ofree);
         } while (w.next(a));
     }
-
     __syncwarp();
     __syncthreads();
     if (tid == 0 && (ctl.stop || (ptx::smem_u32(sm) & 1023))) flag(a.status, ST_TIMEOUT);
