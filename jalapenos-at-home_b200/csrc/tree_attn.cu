@@ -191,15 +191,14 @@ __global__ void __launch_bounds__(CC_T) k_tree_attn_cc(Args a) {
 // The rows to add (query rows of the items that ws_join names) are dealt out
 // over all blocks: each block scans the at most CB_MOST entries into a list of
 // items and the groups of rows before each, then takes every gridDim.x-th
-// group.  Lane l of a warp holds dims 4 l .. of a row.  An item of few partials
-// has groups of CB_ROWS rows, CB_ROWS / CB_WARPS of them to a warp at once; one
-// of many has groups of one row, whose partials the warps share and add in
-// order.
-constexpr int CB_WARPS = 4, CB_T = 32 * CB_WARPS;
-constexpr int CB_MOST = 512;   // workers at most
+// group.  Lane l of a warp holds dims 4 l .. of a row, and all partials it adds
+// are in flight at once where they are few: an item of fewer than CB_SHARE
+// partials has groups of CB_ROWS rows, CB_RPW to a warp; one of more has groups
+// of one row, whose partials the warps share and add in order.
+constexpr int CB_WARPS = 4, CB_T = 32 * CB_WARPS, CB_PER_SM = 5;
+constexpr int CB_MOST = 512, CB_EACH = CB_MOST / CB_T;  // workers at most; of them to a thread
 constexpr int CB_SHARE = 8;    // partials from which the warps share a row
-constexpr int CB_AHEAD = 8;    // loads in flight
-constexpr int CB_ROWS = 16, CB_RPW = CB_ROWS / CB_WARPS;
+constexpr int CB_RPW = 2, CB_ROWS = CB_RPW * CB_WARPS;
 
 struct RowSum {
     float top, sum;
@@ -215,54 +214,57 @@ __device__ __forceinline__ void add_part(RowSum& t, float m, float l, float4 v) 
 }
 
 template <typename T>
-__global__ void __launch_bounds__(CB_T) k_tree_combine(Args a) {
+__global__ void __launch_bounds__(CB_T, CB_PER_SM) k_tree_combine(Args a) {
     __shared__ float4 share_o[CB_WARPS][32];
     __shared__ float2 share_ml[CB_WARPS];
     __shared__ int before[CB_MOST + 1];  // groups of CB_WARPS rows before item i
     __shared__ short who[CB_MOST];       // item i is ws_join[who[i]]
-    __shared__ int warp_items[CB_WARPS], warp_groups[CB_WARPS];
+    __shared__ int2 warp_sums[CB_WARPS];
     const int t = threadIdx.x, warp = t >> 5, l = t & 31;
     ptx::grid_dependency_wait();
     ptx::launch_dependents();
-    // items and their groups of rows, over all tiles (the last may be short)
-    int items = 0, groups = 0;
-    for (int w0 = 0; w0 < a.workers; w0 += CB_T) {
-        const int w = w0 + t;
+    // items and their groups of rows: thread t's workers are CB_EACH t ..
+    int some = 0, groups = 0, mine[CB_EACH];
+#pragma unroll
+    for (int e = 0; e < CB_EACH; ++e) {
+        const int w = t * CB_EACH + e;
         const int4 join = w > 0 && w < a.workers ? a.ws_join[w] : make_int4(0, 0, 0, 0);
-        const int rows = join.w > 0 ? join.y * a.group : 0, g = join.w >= CB_SHARE ? rows : (rows + CB_ROWS - 1) / CB_ROWS;
-        const unsigned some = __ballot_sync(0xffffffffu, g > 0);
-        int inc = g;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int up = __shfl_up_sync(0xffffffffu, inc, o);
-            if (l >= o) inc += up;
-        }
-        if (l == 31) {
-            warp_items[warp] = __popc(some);
-            warp_groups[warp] = inc;
-        }
-        __syncthreads();
-        int at = items + __popc(some & ((1u << l) - 1)), sum = groups + inc - g;
-#pragma unroll
-        for (int i = 0; i < CB_WARPS; ++i) {
-            if (i < warp) {
-                at += warp_items[i];
-                sum += warp_groups[i];
-            }
-            items += warp_items[i];
-            groups += warp_groups[i];
-        }
-        if (g > 0) {
-            who[at] = (short)w;
-            before[at] = sum;
-        }
-        __syncthreads();
+        const int rows = join.w > 0 ? join.y * a.group : 0;
+        mine[e] = join.w >= CB_SHARE ? rows : (rows + CB_ROWS - 1) / CB_ROWS;
     }
-    if (t == 0) before[items] = groups;
+#pragma unroll
+    for (int e = 0; e < CB_EACH; ++e) {
+        some += mine[e] > 0;
+        groups += mine[e];
+    }
+    int item = some, sum = groups;  // up to and with this thread's
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, item, o), up2 = __shfl_up_sync(0xffffffffu, sum, o);
+        if (l >= o) item += up, sum += up2;
+    }
+    if (l == 31) warp_sums[warp] = make_int2(item, sum);
+    __syncthreads();
+    item -= some;
+    sum -= groups;
+    groups = 0;
+#pragma unroll
+    for (int i = 0; i < CB_WARPS; ++i) {
+        if (i < warp) item += warp_sums[i].x, sum += warp_sums[i].y;
+        groups += warp_sums[i].y;
+    }
+#pragma unroll
+    for (int e = 0; e < CB_EACH; ++e)
+        if (mine[e] > 0) {
+            who[item] = (short)(t * CB_EACH + e);
+            before[item++] = sum;
+            sum += mine[e];
+        }
+    if (t == CB_T - 1) before[item] = groups;
     __syncthreads();
     const float inv_group = 1.f / a.group;
     const int R = a.tile_rows;
-    int item = 0;
+    item = 0;
     for (int i = blockIdx.x; i < groups; i += gridDim.x) {
         while (before[item + 1] <= i) ++item;
         const int w = who[item];
@@ -283,45 +285,40 @@ __global__ void __launch_bounds__(CB_T) k_tree_combine(Args a) {
                     sum.sum == 0.f ? -INFINITY : (sum.top + log2f(sum.sum)) * LN2;
         };
         if (parts < CB_SHARE) {
-            RowSum sum[CB_RPW];
-            int g[CB_RPW];
+            float2 ml[CB_RPW][CB_SHARE - 1];
+            float4 v[CB_RPW][CB_SHARE - 1];
 #pragma unroll
             for (int r = 0; r < CB_RPW; ++r) {
-                g[r] = at * CB_ROWS + r * CB_WARPS + warp;
-                sum[r] = RowSum{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
-            }
-            for (int x = 0; x < parts; x += 2) {
-                float2 ml[CB_RPW][2];
-                float4 v[CB_RPW][2];
+                const int g = at * CB_ROWS + r * CB_WARPS + warp;
 #pragma unroll
-                for (int r = 0; r < CB_RPW; ++r)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        ml[r][e] = make_float2(-INFINITY, 0.f);
-                        v[r][e] = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (x + e < parts && g[r] < rows) {
-                            const size_t p = slot(x + e, g[r]);
-                            ml[r][e] = *(const float2*)(a.ws_ml + p * 2);
-                            v[r][e] = *(const float4*)(a.ws_o + p * HEAD + 4 * l);
-                        }
+                for (int x = 0; x < CB_SHARE - 1; ++x) {
+                    ml[r][x] = make_float2(-INFINITY, 0.f);
+                    v[r][x] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (x < parts && g < rows) {
+                        const size_t p = slot(x, g);
+                        ml[r][x] = *(const float2*)(a.ws_ml + p * 2);
+                        v[r][x] = *(const float4*)(a.ws_o + p * HEAD + 4 * l);
                     }
-#pragma unroll
-                for (int r = 0; r < CB_RPW; ++r)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) add_part(sum[r], ml[r][e].x, ml[r][e].y, v[r][e]);
+                }
             }
 #pragma unroll
-            for (int r = 0; r < CB_RPW; ++r)
-                if (g[r] < rows) finish(sum[r], g[r]);
+            for (int r = 0; r < CB_RPW; ++r) {
+                const int g = at * CB_ROWS + r * CB_WARPS + warp;
+                RowSum sum{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+#pragma unroll
+                for (int x = 0; x < CB_SHARE - 1; ++x)
+                    if (x < parts) add_part(sum, ml[r][x].x, ml[r][x].y, v[r][x]);
+                if (g < rows) finish(sum, g);
+            }
             continue;
         }
         const int x0 = parts * warp / CB_WARPS, x1 = parts * (warp + 1) / CB_WARPS;
         RowSum sum{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
-        for (int x = x0; x < x1; x += CB_AHEAD) {
-            float2 ml[CB_AHEAD];
-            float4 v[CB_AHEAD];
+        for (int x = x0; x < x1; x += CB_SHARE) {
+            float2 ml[CB_SHARE];
+            float4 v[CB_SHARE];
 #pragma unroll
-            for (int e = 0; e < CB_AHEAD; ++e) {
+            for (int e = 0; e < CB_SHARE; ++e) {
                 ml[e] = make_float2(-INFINITY, 0.f);
                 v[e] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (x + e < x1) {
@@ -331,7 +328,7 @@ __global__ void __launch_bounds__(CB_T) k_tree_combine(Args a) {
                 }
             }
 #pragma unroll
-            for (int e = 0; e < CB_AHEAD; ++e) add_part(sum, ml[e].x, ml[e].y, v[e]);
+            for (int e = 0; e < CB_SHARE; ++e) add_part(sum, ml[e].x, ml[e].y, v[e]);
         }
         __syncthreads();  // the last row's sums were read
         share_o[warp][l] = sum.o;
@@ -464,7 +461,7 @@ jl_status tree_attention(const jl_tree_attn& a, cudaStream_t st) {
     if (p.workers > 1) {
         // all blocks resident, at most one per row there may be
         const long long most = (long long)(p.workers - 1) * a.max_nodes * k.group;
-        const dim3 grid((unsigned)std::min<long long>(8ll * on.sms, most));
+        const dim3 grid((unsigned)std::min<long long>((long long)CB_PER_SM * on.sms, most));
         JL_TRY((f ? launch_pdl(k_tree_combine<float>, grid, dim3(CB_T), 0, st, k)
                   : launch_pdl(k_tree_combine<uint16_t>, grid, dim3(CB_T), 0, st, k)));
     }
