@@ -70,39 +70,76 @@ __device__ __forceinline__ long long place(const CompactArgs& a, int s, long lon
     return ((long long)page * a.kv_heads * PAGE + p % PAGE) * a.row_bytes;
 }
 
-// Block (kv head, 2 * layer + K|V, sequence): every row of the path is read
-// into shared memory before any is written, so the order of the path and
-// repeated entries do not matter.
-constexpr int CP_T = 128;
-__global__ void __launch_bounds__(CP_T) k_kv_compact(CompactArgs a) {
+// Block (y, sequence): a warp moves the rows of one slab (a kv head's K or V of
+// one layer) after the other.  BATCH rows are read into registers before any of
+// them is written; with at most BATCH rows the order of the path and repeated
+// entries then do not matter.  A longer path is moved batch by batch, which is
+// right as long as no batch reads a row that an earlier one wrote (a tree's
+// path: entry i is node i or later); a path that does (or may) goes through
+// shared memory whole, slab by slab.  The places of the rows are looked up once
+// a block.  Bound by memory for many slabs and by the lookups' latency for few:
+// B200, 36 layers of 8 heads, 32 sequences of 5 to 9 rows 16.3 us (4.3 TB/s of
+// scattered 256-byte rows), one sequence of 4 rows 2.6 us.
+constexpr int CP_WARPS = 4, CP_T = 32 * CP_WARPS, CP_BATCH = 16;
+
+template <int ROW_BYTES>
+__global__ void __launch_bounds__(CP_T) k_kv_compact(CompactArgs a, int slabs, int per_block) {
+    constexpr int CHUNKS = ROW_BYTES / 16, REGS = CP_BATCH * CHUNKS / 32;
     extern __shared__ uint4 cp_rows[];
     __shared__ long long from[JL_TREE_MAX_NODES], to[JL_TREE_MAX_NODES];
     ptx::grid_dependency_wait();
     ptx::launch_dependents();
-    const int s = blockIdx.z, head = blockIdx.x;
-    uint8_t* base = (blockIdx.y & 1 ? a.v : a.k) + (size_t)(blockIdx.y >> 1) * a.layer_stride +
-                    (size_t)head * PAGE * a.row_bytes;
+    const int s = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int n = a.path_len[s];
     int bad = n < 0 || n > a.path_ld ? 2 : 0;
     n = min(max(n, 0), a.path_ld);
+    bool back = false;  // an entry reads what an earlier batch may write
     for (int i = threadIdx.x; i < n; i += CP_T) {
         const long long c = a.ctx[s], p = a.path[(size_t)s * a.path_ld + i];
         const bool neg = c < 0 || p < 0;
         if (neg) bad |= 2;
         from[i] = neg ? -1 : place(a, s, c + p, &bad);
         to[i] = neg || p == i ? -1 : place(a, s, c + i, &bad);
+        if (from[i] < 0 || to[i] < 0) from[i] = -1;
+        // never within the first batch, so paths of one batch need no shared memory
+        back |= from[i] >= 0 && p < i / CP_BATCH * CP_BATCH;
     }
     if (bad && a.status) atomicOr(a.status, bad);
-    __syncthreads();
-    const int chunks = a.row_bytes / 16;  // 16 or 32
-    for (int i = threadIdx.x; i < n * chunks; i += CP_T) {
-        const int r = i / chunks, c = i % chunks;
-        if (from[r] >= 0 && to[r] >= 0) cp_rows[i] = *(const uint4*)(base + from[r] + 16 * c);
+    back = __syncthreads_or(back);
+    const int slab0 = blockIdx.x * per_block, slab1 = min(slabs, slab0 + per_block);
+    auto base_of = [&](int slab) {  // slab = (2 * layer + K|V) * kv_heads + head
+        const int lk = slab / a.kv_heads;
+        return (lk & 1 ? a.v : a.k) + (size_t)(lk >> 1) * a.layer_stride + (size_t)(slab - lk * a.kv_heads) * PAGE * ROW_BYTES;
+    };
+    if (back) {
+        for (int slab = slab0; slab < slab1; ++slab) {
+            uint8_t* base = base_of(slab);
+            for (int i = threadIdx.x; i < n * CHUNKS; i += CP_T)
+                if (from[i / CHUNKS] >= 0) cp_rows[i] = *(const uint4*)(base + from[i / CHUNKS] + 16 * (i % CHUNKS));
+            __syncthreads();
+            for (int i = threadIdx.x; i < n * CHUNKS; i += CP_T)
+                if (from[i / CHUNKS] >= 0) *(uint4*)(base + to[i / CHUNKS] + 16 * (i % CHUNKS)) = cp_rows[i];
+            __syncthreads();
+        }
+        return;
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < n * chunks; i += CP_T) {
-        const int r = i / chunks, c = i % chunks;
-        if (from[r] >= 0 && to[r] >= 0) *(uint4*)(base + to[r] + 16 * c) = cp_rows[i];
+    for (int slab = slab0 + warp; slab < slab1; slab += CP_WARPS) {
+        uint8_t* base = base_of(slab);
+        for (int r0 = 0; r0 < n; r0 += CP_BATCH) {
+            uint4 v[REGS];
+#pragma unroll
+            for (int k = 0; k < REGS; ++k) {
+                const int i = k * 32 + lane, r = r0 + i / CHUNKS;
+                if (r < n && from[r] >= 0) v[k] = *(const uint4*)(base + from[r] + 16 * (i % CHUNKS));
+            }
+            __syncwarp();  // all lanes have read before one writes
+#pragma unroll
+            for (int k = 0; k < REGS; ++k) {
+                const int i = k * 32 + lane, r = r0 + i / CHUNKS;
+                if (r < n && from[r] >= 0) *(uint4*)(base + to[r] + 16 * (i % CHUNKS)) = v[k];
+            }
+            __syncwarp();
+        }
     }
 }
 
@@ -116,7 +153,8 @@ struct CopyList {
 
 constexpr int CY_T = 256;
 // Block (kv head, pair, 2 * layer + K|V): one head's rows of a page, which lie
-// together (16 KB in bf16).
+// together (16 KB in bf16).  Bound by memory: B200, 64 pages of 8 heads in 36
+// layers, 166 us (6.8 TB/s read and written, the measured copy rate).
 template <int N>
 __global__ void __launch_bounds__(CY_T) k_kv_copy(uint8_t* k, uint8_t* v, size_t layer_stride, int kv_heads, int row_bytes,
                                                   const __grid_constant__ CopyList<N> list) {
@@ -159,11 +197,20 @@ jl_status kv_compact(const jl_kv_compaction& a, cudaStream_t st) {
     const int row_bytes = HEAD * (a.pool.dtype == JL_KV_F32 ? 4 : 2);
     CompactArgs k{(uint8_t*)a.pool.k, (uint8_t*)a.pool.v, a.pool.layer_stride, a.pool.kv_heads, a.pool.pages, a.seqs,
                   a.path_ld, a.max_pages, row_bytes, a.ctx, a.path, a.path_len, a.page_table, a.status};
-    const size_t smem = (size_t)a.path_ld * row_bytes;
-    if (smem > 40 * 1024)  // the default limit is 48 KB with the static arrays
-        JL_CUDA(cudaFuncSetAttribute(k_kv_compact, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     JL_TREE_MAX_NODES * HEAD * 4));
-    return launch_pdl(k_kv_compact, dim3(a.pool.kv_heads, 2 * a.pool.layers, a.seqs), dim3(CP_T), smem, st, k);
+    // paths of one batch need no shared memory
+    const size_t smem = a.path_ld > CP_BATCH ? (size_t)a.path_ld * row_bytes : 0;
+    const int slabs = 2 * a.pool.layers * a.pool.kv_heads;
+    // a slab a warp for few slabs; for many, what the resident warps share
+    const long long warps = (long long)on.sms * 8 * CP_WARPS;
+    const int per_warp = (int)std::max<long long>(1, (long long)slabs * a.seqs / warps);
+    const int per_block = per_warp * CP_WARPS;
+    const dim3 grid((slabs + per_block - 1) / per_block, a.seqs);
+    auto go = [&](auto kernel) -> jl_status {
+        if (smem > 40 * 1024)  // the default limit is 48 KB with the static arrays
+            JL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, JL_TREE_MAX_NODES * HEAD * 4));
+        return launch_pdl(kernel, grid, dim3(CP_T), smem, st, k, slabs, per_block);
+    };
+    return row_bytes == 256 ? go(k_kv_compact<256>) : go(k_kv_compact<512>);
 }
 
 jl_status kv_copy_pages(const jl_kv_pages& pool, const int32_t* src, const int32_t* dst, const int32_t* rows, size_t n,

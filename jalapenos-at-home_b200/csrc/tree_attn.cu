@@ -43,7 +43,7 @@ constexpr size_t cc_smem() {
 }
 
 template <typename T, int RT>
-__global__ void __launch_bounds__(CC_T) k_tree_attn_cc(Args a) {
+__global__ void __launch_bounds__(CC_T, RT <= 2 ? 2 : 1) k_tree_attn_cc(Args a) {
     extern __shared__ __align__(16) float cc_smem_raw[];
     float* qs = cc_smem_raw;                  // [16 RT][CC_KLD]
     float* ks = qs + 16 * RT * CC_KLD;        // [PAGE][CC_KLD]
@@ -88,15 +88,22 @@ __global__ void __launch_bounds__(CC_T) k_tree_attn_cc(Args a) {
             const int used = there ? (int)min((long long)PAGE, (long long)w.q.ctx + w.q.n - (long long)p * PAGE) : 0;
             __syncthreads();  // the previous page's tiles are no longer read
             const size_t at = kv_index(there ? page : 0, w.h, 0, a.kv_heads);
-            for (int i = tid; i < PAGE * 32; i += CC_T) {
-                const int r = i >> 5, c = i & 31;
-                float4 kk = make_float4(0.f, 0.f, 0.f, 0.f), vv = kk;
+            constexpr int LOADS = PAGE * 32 / CC_T;
+            float4 kk[LOADS], vv[LOADS];  // all in flight
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                const int r = (tid + i * CC_T) >> 5, c = tid & 31;
+                kk[i] = vv[i] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (r < used) {  // rows past the sequence may hold anything
-                    kk = load4((const float*)a.k + at + (size_t)r * HEAD + 4 * c);
-                    vv = load4((const float*)a.v + at + (size_t)r * HEAD + 4 * c);
+                    kk[i] = load4((const float*)a.k + at + (size_t)r * HEAD + 4 * c);
+                    vv[i] = load4((const float*)a.v + at + (size_t)r * HEAD + 4 * c);
                 }
-                *(float4*)(ks + r * CC_KLD + 4 * c) = kk;
-                *(float4*)(vs + r * HEAD + 4 * c) = vv;
+            }
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                const int r = (tid + i * CC_T) >> 5, c = tid & 31;
+                *(float4*)(ks + r * CC_KLD + 4 * c) = kk[i];
+                *(float4*)(vs + r * HEAD + 4 * c) = vv[i];
             }
             __syncthreads();
             const bool edge = (long long)(p + 1) * PAGE > w.q.ctx || !there;
@@ -104,6 +111,8 @@ __global__ void __launch_bounds__(CC_T) k_tree_attn_cc(Args a) {
 #pragma unroll
             for (int j = 0; j < RT; ++j) {
                 const int r = ty + 16 * j;
+                vis[j] = 0;
+                if (16 * j + (ty & ~1) >= live) break;  // neither row of the warp is live
                 vis[j] = !there || r >= live ? 0 : edge ? visible(a, w.q, (lane * R + r) / a.group, p) : ~0ull;
                 float sc[4] = {0.f, 0.f, 0.f, 0.f};
                 const float* qr = qs + r * CC_KLD;
@@ -146,6 +155,7 @@ __global__ void __launch_bounds__(CC_T) k_tree_attn_cc(Args a) {
                 const float4 v1 = *(const float4*)(vs + key * HEAD + 64 + 4 * tx);
 #pragma unroll
                 for (int j = 0; j < RT; ++j) {
+                    if (16 * j + (ty & ~1) >= live) break;
                     // not seen: skipped, not multiplied by zero (V may be infinite)
                     if (edge && !(vis[j] >> key & 1)) continue;
                     const float e = ps[(ty + 16 * j) * CC_PLD + key];
@@ -354,9 +364,9 @@ Plan plan_of(const jl_tree_attn& a, int sms) {
     Plan p;
     const int rows = a.max_nodes * (a.q_heads / a.pool.kv_heads);
     const bool tc = a.pool.dtype == JL_KV_BF16;
-    p.tile_rows = tc ? tc_tile_rows(a.dtype == JL_KV_F32) : rows <= 16 ? 16 : 64;
+    p.tile_rows = tc ? tc_tile_rows(a.dtype == JL_KV_F32) : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
     p.lanes = (rows + p.tile_rows - 1) / p.tile_rows;
-    p.workers = std::min(CB_MOST, std::max(1, (tc ? TC_CTAS_PER_SM : 1) * sms / p.lanes));
+    p.workers = std::min(CB_MOST, std::max(1, (tc ? TC_CTAS_PER_SM : p.tile_rows <= 32 ? 2 : 1) * sms / p.lanes));
     p.min_units = 1 + SEG;
     p.bytes = p.workers == 1 ? 0 : (size_t)p.workers * (sizeof(int4) + (size_t)p.lanes * 2 * p.tile_rows * (HEAD + 2) * sizeof(float));
     return p;
@@ -366,12 +376,14 @@ template <typename T>
 jl_status launch_cc(const Args& a, cudaStream_t st) {
     const dim3 grid(a.workers, a.lanes);
     if (a.tile_rows == 16) return launch_pdl(k_tree_attn_cc<T, 1>, grid, dim3(CC_T), cc_smem<1>(), st, a);
+    if (a.tile_rows == 32) return launch_pdl(k_tree_attn_cc<T, 2>, grid, dim3(CC_T), cc_smem<2>(), st, a);
     return launch_pdl(k_tree_attn_cc<T, 4>, grid, dim3(CC_T), cc_smem<4>(), st, a);
 }
 
 template <typename T>
 jl_status configure_cc() {
     JL_CUDA(cudaFuncSetAttribute(k_tree_attn_cc<T, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cc_smem<1>()));
+    JL_CUDA(cudaFuncSetAttribute(k_tree_attn_cc<T, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cc_smem<2>()));
     JL_CUDA(cudaFuncSetAttribute(k_tree_attn_cc<T, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cc_smem<4>()));
     return JL_OK;
 }
