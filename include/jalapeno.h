@@ -149,6 +149,20 @@ size_t jl_cache_len(const jl_cache* c);
 /* len must not exceed the current length (KvCache::truncate asserts). */
 jl_status jl_cache_truncate(jl_cache* c, size_t len);
 
+/* A new cache that continues from the first `len` positions of `c` (at most
+ * its length).  The two share full pages, and the page that `len` ends in is
+ * copied; a cache that later writes into a shared page (after a truncation)
+ * first gets a copy of its own, so neither sees the other's tokens.  Pages go
+ * back to the pool with the last cache that holds them.  No counterpart in the
+ * reference, whose caches are contiguous. */
+jl_status jl_cache_fork(jl_cache* c, size_t len, jl_cache** out);
+/* After jl_predict_tree: keeps `n` of the tree's nodes, a path from a child of
+ * the committed positions down (each entry a child of the one before it), moves
+ * their keys and values together and adds them to the length.  n == 0 keeps
+ * none.  Any other pass on the cache, a truncation or this call drops the rest
+ * of the tree. */
+jl_status jl_cache_compact(jl_cache* c, const uint32_t* path, size_t n);
+
 /* ------------------------------------------------------------------------
  * Forward passes: Model::predict / next_token / hidden (model.rs:143-240),
  * GpuModel::run (gpu.rs:544-634).  One host sync per call.
@@ -168,6 +182,17 @@ jl_status jl_predict(jl_model* m, jl_cache* c, const uint32_t* ids, size_t n, in
  * Model::predict); it lets callers check those kernels' logits. */
 jl_status jl_predict_draft(jl_model* m, jl_cache* c, const uint32_t* ids, size_t n,
                            uint32_t* out_id, float* out_logits);
+/* Verifies a tree of drafted tokens in one pass: node i holds ids[i] and
+ * follows node parents[i] (an earlier node, or -1: the committed positions), and
+ * out_ids[i] is the model's next token after the committed positions and node
+ * i's path.  A chain (parents -1, 0, 1, ..) predicts what jl_predict with `all`
+ * set does, up to the rounding of other kernels (logits within 2e-4 relative L2
+ * on a bf16 pool).  1..JL_TREE_MAX_NODES nodes, at most max_pass_rows, and
+ * length + n within the context limit.  The length stays; jl_cache_compact
+ * keeps a path.  The reference verifies chains only (speculative.rs:95-97).
+ * out_logits (nullable) receives [n, vocab] f32 logits. */
+jl_status jl_predict_tree(jl_model* m, jl_cache* c, const uint32_t* ids, const int32_t* parents, size_t n,
+                          uint32_t* out_ids, float* out_logits);
 /* Model::next_token (model.rs:203-205): predict after a fresh prompt. */
 jl_status jl_next_token(jl_model* m, const uint32_t* ids, size_t n, uint32_t* out_id);
 /* Model::hidden (model.rs:143-154): residual stream after `layers` layers

@@ -245,7 +245,22 @@ jl_status jl_cache_truncate(jl_cache* c, size_t len) {
     // KvCache::truncate asserts len <= self.len (engine/src/model.rs:46)
     JL_NEED(len <= c->len, "truncate length exceeds the cache length");
     c->len = len;
+    c->tree.clear();
     return JL_OK;
+}
+
+jl_status jl_cache_fork(jl_cache* c, size_t len, jl_cache** out) {
+    JL_NEED(c && out, "cache and out must be non-null");
+    *out = nullptr;
+    JL_NEED(c->m, "the cache's model was freed");
+    JL_NEED(len <= c->len, "fork length exceeds the cache length");
+    JL_GUARD({ return cache_fork(c, len, out); })
+}
+
+jl_status jl_cache_compact(jl_cache* c, const uint32_t* path, size_t n) {
+    JL_NEED(c && (path || !n), "cache and path must be non-null");
+    JL_NEED(c->m, "the cache's model was freed");
+    JL_GUARD({ return cache_compact(c, path, n); })
 }
 
 // ---- passes ------------------------------------------------------------------
@@ -263,6 +278,13 @@ jl_status jl_predict_draft(jl_model* m, jl_cache* c, const uint32_t* ids, size_t
     JL_NEED(c->m == m, "this cache belongs to another model");
     JL_NEED(n == 1 || n == 2, "a draft step takes 1 or 2 tokens");
     JL_GUARD({ return predict(m, c, ids, n, false, out_id, out_logits, true); })
+}
+
+jl_status jl_predict_tree(jl_model* m, jl_cache* c, const uint32_t* ids, const int32_t* parents, size_t n,
+                          uint32_t* out_ids, float* out_logits) {
+    JL_NEED(m && c && ids && parents && out_ids, "model, cache, ids, parents and out_ids must be non-null");
+    JL_NEED(c->m == m, "this cache belongs to another model");
+    JL_GUARD({ return predict_tree(m, c, ids, parents, n, out_ids, out_logits); })
 }
 
 jl_status jl_next_token(jl_model* m, const uint32_t* ids, size_t n, uint32_t* out_id) {

@@ -460,6 +460,7 @@ jl_status predict_start(jl_model* m, jl_cache* c, const uint32_t* ids, size_t n,
     JL_TRY(check_ids(m, ids, n));
     JL_CUDA(cudaSetDevice(m->device));
     JL_TRY(cache_reserve(c, c->len + n, m->stream));
+    c->tree.clear();  // the pass writes over the nodes of a tree pass
     // The captured decode pass takes 16 rows at a time (the kernels are
     // row-count invariant, so chunking changes no result).  On a model whose
     // pass is fused onto the tensor cores it is faster than the tiled

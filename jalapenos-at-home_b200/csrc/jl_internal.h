@@ -228,11 +228,13 @@ struct KvPool {
     size_t pages = 0;
     void* base = nullptr;                 // [layers][2][pages][kv_heads][PAGE][HEAD]
     std::vector<int32_t> free_list;
+    std::vector<int32_t> refs;            // caches that hold each page (forks share pages)
     size_t page_elems = 0;                // kv_heads * PAGE * HEAD
 };
 
 struct SpecGraph;   // device-resident speculative loop (engine.cu)
 struct BatchGraph;  // device-resident loop over a batch of sequences (batch.cu)
+struct TreeBuffers;  // descriptors and workspace of tree passes (tree_pass.cu)
 
 }  // namespace jl
 
@@ -287,6 +289,7 @@ struct jl_model {
     std::vector<jl::SpecGraph*> spec_graphs;  // owned; freed by model_free
     std::vector<jl::BatchGraph*> batch_graphs;  // owned; freed by model_free
     std::vector<jl_cache*> caches;              // live caches; detached by model_free
+    jl::TreeBuffers* tree = nullptr;            // owned; made by the first tree pass
     int* counters = nullptr;              // zeroed split-K / reduction counters
     std::map<std::string, std::pair<const void*, size_t>> tensor_index;  // name -> device bytes
 };
@@ -305,6 +308,9 @@ struct jl_cache {
     int32_t* h_pages = nullptr;           // pinned mirror
     size_t max_pages = 0;
     size_t len = 0;
+    // parents of the nodes that a tree pass left behind len, until another pass
+    // writes there or a path of them is kept
+    std::vector<int32_t> tree;
 };
 
 namespace jl {
@@ -317,6 +323,17 @@ void model_free(jl_model* m);
 jl_status cache_create(jl_model* m, jl_cache** out);
 void cache_free(jl_cache* c);
 jl_status cache_reserve(jl_cache* c, size_t tokens, cudaStream_t stream);
+// A free page, held by its taker; and the end of one hold on a page.
+jl_status page_take(jl_model* m, int32_t* page);
+void page_release(jl_model* m, int32_t page);
+
+// ---- trees of drafted tokens and forks (tree_pass.cu) --------------------------
+jl_status predict_tree(jl_model* m, jl_cache* c, const uint32_t* ids, const int32_t* parents, size_t n,
+                       uint32_t* out_ids, float* out_logits);
+jl_status cache_compact(jl_cache* c, const uint32_t* path, size_t n);
+jl_status cache_fork(jl_cache* c, size_t len, jl_cache** out);
+jl_status page_unshare(jl_cache* c, size_t i, size_t rows, cudaStream_t stream);
+void tree_buffers_free(TreeBuffers* t);
 
 // ---- passes and generation (engine.cu) ---------------------------------------
 // Records the kernels of one forward pass on `stream`.  rows_cap bounds the

@@ -96,6 +96,7 @@ jl_status finish_model(jl_model* m, const jl_model_options& o) {
     }
     JL_TRY(kv_tensor_maps(m));  // the tensor-core prompt attention's TMA view of the pool
     m->kv.free_list.resize(m->kv.pages);
+    m->kv.refs.assign(m->kv.pages, 0);
     for (size_t i = 0; i < m->kv.pages; ++i) m->kv.free_list[i] = (int32_t)(m->kv.pages - 1 - i);
     // decode attention over long contexts: the partial sums of up to
     // ATT_ZMAX window CTAs for every row of the largest multi-chunk pass
@@ -696,6 +697,7 @@ void model_free(jl_model* m) {
     cudaFree(m->mx.scratch);
     cudaFree(m->att_ws);
     cudaFree(m->att_cnt);
+    tree_buffers_free(m->tree);
     for (StageSlot& sl : m->stage) {
         if (sl.done) cudaEventDestroy(sl.done);
         cudaFreeHost(sl.hdr);
@@ -736,7 +738,7 @@ void cache_free(jl_cache* c) {
         jl_model* m = c->m;
         cudaSetDevice(m->device);
         if (m->stream) cudaStreamSynchronize(m->stream);
-        for (int32_t p : c->pages) m->kv.free_list.push_back(p);
+        for (int32_t p : c->pages) page_release(m, p);
         m->caches.erase(std::remove(m->caches.begin(), m->caches.end(), c), m->caches.end());
     }
     cudaFree(c->d_pages);
@@ -745,29 +747,51 @@ void cache_free(jl_cache* c) {
     delete c;
 }
 
-// Makes sure pages exist for positions [0, tokens).  New page-table entries
-// are copied to the device on `stream`, ahead of the pass that uses them.
+jl_status page_take(jl_model* m, int32_t* page) {
+    auto& fl = m->kv.free_list;
+    if (fl.empty()) {
+        set_error("KV pool exhausted: need 1 more page, 0 free (raise kv_pool_tokens)");
+        return JL_ERR_OOM;
+    }
+    *page = fl.back();
+    fl.pop_back();
+    m->kv.refs[*page] = 1;
+    return JL_OK;
+}
+
+void page_release(jl_model* m, int32_t page) {
+    if (--m->kv.refs[page] == 0) m->kv.free_list.push_back(page);
+}
+
+// Makes sure pages exist for positions [0, tokens), and that those from the
+// cache's length on, which a pass may write, are its own: a page shared with a
+// fork is replaced by a copy of the rows before the length.  New page-table
+// entries are copied to the device on `stream`, ahead of the pass that uses them.
 jl_status cache_reserve(jl_cache* c, size_t tokens, cudaStream_t stream) {
-    const size_t need = (tokens + PAGE - 1) / PAGE;
-    if (need <= c->pages.size()) return JL_OK;
+    const size_t need = (tokens + PAGE - 1) / PAGE, have = c->pages.size();
     if (need > c->max_pages) {
         set_error("sequence of %zu tokens exceeds the context limit", tokens);
         return JL_ERR_INVALID_ARG;
     }
-    auto& fl = c->m->kv.free_list;
-    if (need - c->pages.size() > fl.size()) {
-        set_error("KV pool exhausted: need %zu more pages, %zu free (raise kv_pool_tokens)",
-                  need - c->pages.size(), fl.size());
+    jl_model* m = c->m;
+    const size_t keep = c->len / PAGE;
+    size_t fresh = need > have ? need - have : 0;
+    for (size_t i = keep; i < std::min(need, have); ++i) fresh += m->kv.refs[c->pages[i]] > 1;
+    if (fresh > m->kv.free_list.size()) {
+        set_error("KV pool exhausted: need %zu more pages, %zu free (raise kv_pool_tokens)", fresh, m->kv.free_list.size());
         return JL_ERR_OOM;
     }
-    const size_t first = c->pages.size();
+    for (size_t i = keep; i < std::min(need, have); ++i)
+        if (m->kv.refs[c->pages[i]] > 1) JL_TRY(page_unshare(c, i, i == keep ? c->len % PAGE : 0, stream));
+    if (need <= have) return JL_OK;
     while (c->pages.size() < need) {
-        c->h_pages[c->pages.size()] = fl.back();
-        c->pages.push_back(fl.back());
-        fl.pop_back();
+        int32_t page = 0;
+        JL_TRY(page_take(m, &page));
+        c->h_pages[c->pages.size()] = page;
+        c->pages.push_back(page);
     }
-    JL_CUDA(cudaMemcpyAsync(c->d_pages + first, c->h_pages + first, (need - first) * sizeof(int32_t),
-                            cudaMemcpyHostToDevice, stream));
+    JL_CUDA(cudaMemcpyAsync(c->d_pages + have, c->h_pages + have, (need - have) * sizeof(int32_t), cudaMemcpyHostToDevice,
+                            stream));
     return JL_OK;
 }
 

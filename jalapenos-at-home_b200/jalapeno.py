@@ -41,7 +41,7 @@ EXPORTS = (
     "jl_project_noalloc", "jl_pass_kernels", "jl_time_pass_draft", "jl_generate_batch",
     "jl_generate_speculative_batch", "jl_timeline_read", "jl_timeline_kernel", "jl_wait_probe",
     "jl_model_prompt_attention", "jl_qk_norm_rope", "jl_tree_attention", "jl_tree_attention_workspace",
-    "jl_kv_compact", "jl_kv_copy_pages",
+    "jl_kv_compact", "jl_kv_copy_pages", "jl_predict_tree", "jl_cache_fork", "jl_cache_compact",
 )
 PROJ_QKV, PROJ_O, PROJ_GATE_UP, PROJ_DOWN, PROJ_HEAD = 0, 1, 2, 3, 4
 
@@ -197,6 +197,9 @@ def _load():
         "jl_timeline_kernel": ([sz], ctypes.c_char_p),
         "jl_wait_probe": ([vp, ctypes.c_uint32], ctypes.c_int),
         "jl_model_prompt_attention": ([vp, ctypes.c_int, ctypes.POINTER(ctypes.c_int)], ctypes.c_int),
+        "jl_predict_tree": ([vp, vp, u32p, ctypes.POINTER(ctypes.c_int32), sz, u32p, f32p], ctypes.c_int),
+        "jl_cache_fork": ([vp, sz, ctypes.POINTER(vp)], ctypes.c_int),
+        "jl_cache_compact": ([vp, u32p, sz], ctypes.c_int),
         "jl_qk_norm_rope": ([ctypes.POINTER(NormRope), vp], ctypes.c_int),
         "jl_tree_attention": ([ctypes.POINTER(TreeAttn), vp], ctypes.c_int),
         "jl_tree_attention_workspace": ([ctypes.POINTER(TreeAttn), ctypes.POINTER(sz)], ctypes.c_int),
@@ -362,6 +365,22 @@ class Model:
         out = [int(i) for i in ids]
         return (out, lg) if logits else out
 
+    def predict_tree(self, tokens, parents, cache: "Cache", logits: bool = False):
+        """Verifies a tree of drafted tokens in one pass: node i follows node
+        ``parents[i]`` (an earlier one, or -1 for the cache's last position);
+        returns the next token after each node's path (jl_predict_tree).
+        ``cache.compact(path)`` then keeps a path of the nodes."""
+        t = u32(tokens)
+        p = np.ascontiguousarray(np.asarray(parents, dtype=np.int32))
+        if p.shape != t.shape:
+            raise ValueError("one parent for each token")
+        out = np.zeros(max(len(t), 1), np.uint32)
+        lg = np.empty((len(t), self.vocab), np.float32) if logits else None
+        check(lib.jl_predict_tree(self._h, cache._h, _p(t, ctypes.c_uint32), _p(p, ctypes.c_int32), len(t),
+                                  _p(out, ctypes.c_uint32), None if lg is None else _p(lg, ctypes.c_float)))
+        ids = [int(i) for i in out[: len(t)]]
+        return (ids, lg) if logits else ids
+
     def predict_draft(self, tokens, cache: "Cache", logits: bool = False):
         """One draft step (1 or 2 tokens, predicting after the last) through
         the kernels a speculative loop's draft passes run: the proposal
@@ -478,11 +497,12 @@ class Model:
 class Cache:
     """``KvCache`` (model.rs:37-52) on the GPU."""
 
-    def __init__(self, model: Model):
+    def __init__(self, model: Model, handle: ctypes.c_void_p | None = None):
         self._model = model
-        h = ctypes.c_void_p()
-        check(lib.jl_cache_create(model._h, ctypes.byref(h)))
-        self._h = h
+        if handle is None:
+            handle = ctypes.c_void_p()
+            check(lib.jl_cache_create(model._h, ctypes.byref(handle)))
+        self._h = handle
 
     def __del__(self):
         if getattr(self, "_h", None):
@@ -495,6 +515,19 @@ class Cache:
 
     def truncate(self, n: int) -> None:
         check(lib.jl_cache_truncate(self._h, n))
+
+    def fork(self, n: int | None = None) -> "Cache":
+        """A cache that continues from this one's first ``n`` positions (all of
+        them by default), sharing full pages with it (jl_cache_fork)."""
+        h = ctypes.c_void_p()
+        check(lib.jl_cache_fork(self._h, self.len if n is None else n, ctypes.byref(h)))
+        return Cache(self._model, h)
+
+    def compact(self, path) -> None:
+        """Keeps a path of the nodes of the last ``predict_tree``
+        (jl_cache_compact)."""
+        p = u32(path)
+        check(lib.jl_cache_compact(self._h, _p(p, ctypes.c_uint32), len(p)))
 
 
 # ---------------------------------------------------------------------------

@@ -109,6 +109,10 @@ def test_null_structures():
     assert J.lib.jl_tree_attention_workspace(None, ctypes.byref(n)) == J.JL_ERR_INVALID_ARG
     assert J.lib.jl_qk_norm_rope(None, None) == J.JL_ERR_INVALID_ARG
     assert J.lib.jl_kv_compact(None, None) == J.JL_ERR_INVALID_ARG
+    out = ctypes.c_void_p()
+    assert J.lib.jl_predict_tree(None, None, None, None, 0, None, None) == J.JL_ERR_INVALID_ARG
+    assert J.lib.jl_cache_fork(None, 0, ctypes.byref(out)) == J.JL_ERR_INVALID_ARG
+    assert J.lib.jl_cache_compact(None, None, 0) == J.JL_ERR_INVALID_ARG
     assert J.lib.jl_kv_copy_pages(None, None, None, None, 0, None) == J.JL_ERR_INVALID_ARG
 
 
