@@ -403,7 +403,7 @@ typedef struct jl_tree_attn {
 } jl_tree_attn;
 jl_status jl_tree_attention(const jl_tree_attn* a, void* stream);
 /* Bytes of workspace the call needs (from its sizes alone; pointers may be
- * NULL except pool.k, which names the device), at most
+ * NULL except pool.k, which names the device; seqs or max_pages 0: for any), at most
  * JL_TREE_WORKSPACE_BYTES. */
 jl_status jl_tree_attention_workspace(const jl_tree_attn* a, size_t* bytes);
 

@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(CC_T, RT <= 2 ? 2 : 1) k_tree_attn_cc(Args a) 
     const Split sp = locate<CC_T>(a, worker, scratch);
     Walk w;
     const bool work = w.start(a, scratch.found, sp.at(worker), sp.at(worker + 1));
-    if (tid == 0 && lane == 0 && a.workers > 1) a.ws_join[worker] = w.join(sp, worker, work);
+    if (tid == 0 && lane == 0 && a.workers > 1 && !a.whole) a.ws_join[worker] = w.join(sp, worker, work);
     if (!work) return;
     do {
         const int live = min(R, w.q.n * a.group - lane * R);  // rows of this tile
@@ -73,10 +73,12 @@ __global__ void __launch_bounds__(CC_T, RT <= 2 ? 2 : 1) k_tree_attn_cc(Args a) 
             *(float4*)(qs + r * CC_KLD + 4 * c) = v;
         }
         float m[RT], l[RT], acc[RT][8];
+        uint64_t m0[RT];
 #pragma unroll
         for (int j = 0; j < RT; ++j) {
             m[j] = -INFINITY;
             l[j] = 0.f;
+            m0[j] = ty + 16 * j < live ? first_word(a, w.q, (lane * R + ty + 16 * j) / a.group) : 0;
 #pragma unroll
             for (int d = 0; d < 8; ++d) acc[j][d] = 0.f;
         }
@@ -113,7 +115,7 @@ __global__ void __launch_bounds__(CC_T, RT <= 2 ? 2 : 1) k_tree_attn_cc(Args a) 
                 const int r = ty + 16 * j;
                 vis[j] = 0;
                 if (16 * j + (ty & ~1) >= live) break;  // neither row of the warp is live
-                vis[j] = !there || r >= live ? 0 : edge ? visible(a, w.q, (lane * R + r) / a.group, p) : ~0ull;
+                vis[j] = !there || r >= live ? 0 : edge ? visible(a, w.q, (lane * R + r) / a.group, p, m0[j]) : ~0ull;
                 float sc[4] = {0.f, 0.f, 0.f, 0.f};
                 const float* qr = qs + r * CC_KLD;
 #pragma unroll 8
@@ -356,7 +358,7 @@ __global__ void __launch_bounds__(CB_T, CB_PER_SM) k_tree_combine(Args a) {
 
 // The kernel that a call takes and how it cuts the work.
 struct Plan {
-    int tile_rows, lanes, workers, min_units;
+    int tile_rows, lanes, workers, min_units, whole;
     size_t bytes;
 };
 
@@ -367,8 +369,21 @@ Plan plan_of(const jl_tree_attn& a, int sms) {
     p.tile_rows = tc ? tc_tile_rows(a.dtype == JL_KV_F32) : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
     p.lanes = (rows + p.tile_rows - 1) / p.tile_rows;
     p.workers = std::min(CB_MOST, std::max(1, (tc ? TC_CTAS_PER_SM : p.tile_rows <= 32 ? 2 : 1) * sms / p.lanes));
-    p.min_units = 1 + SEG;
-    p.bytes = p.workers == 1 ? 0 : (size_t)p.workers * (sizeof(int4) + (size_t)p.lanes * 2 * p.tile_rows * (HEAD + 2) * sizeof(float));
+    // Whole items or split ones: whole, a worker's longest item sets the time (in
+    // waves of all workers); split, the mean does, and the join is added.  The
+    // times, in us on a B200 with every SM busy, are a page's (tensor cores: 1.5
+    // for bf16 rows, 2 for f32; CUDA cores: 8), a segment's start and end (6) and
+    // the join (5).  Measured whole / split, 8 bf16 nodes, 32 heads over 8: one
+    // sequence of 300 positions 10.6 / 14.7 us, 32 of them 15.3 / 30.4 us, 32 of up
+    // to 700 23.6 / 34.5 us; f32 rows, one sequence of 700 29.6 / 20.9 us.
+    const double page = !tc ? 8.0 : a.dtype == JL_KV_F32 ? 2.0 : 1.5;
+    const double ctas = (double)a.seqs * a.pool.kv_heads * p.lanes, slots = (double)p.workers * p.lanes;
+    const double whole = std::ceil(ctas / slots) * (a.max_pages * page + 6);
+    const double split = std::max(ctas * (a.max_pages + SEG) / slots, 1.0 + SEG) * page + 6 + 5;
+    // sizes of 0 ask for the workspace of any call
+    p.whole = a.seqs > 0 && a.max_pages > 0 && whole <= split;
+    p.min_units = p.whole ? 1 : 1 + SEG;
+    p.bytes = p.workers == 1 || p.whole ? 0 : (size_t)p.workers * (sizeof(int4) + (size_t)p.lanes * 2 * p.tile_rows * (HEAD + 2) * sizeof(float));
     return p;
 }
 
@@ -463,6 +478,7 @@ jl_status tree_attention(const jl_tree_attn& a, cudaStream_t st) {
     k.lanes = p.lanes;
     k.tile_rows = p.tile_rows;
     k.min_units = p.min_units;
+    k.whole = p.whole;
     k.ws_join = (int4*)a.workspace;
     k.ws_o = (float*)(k.ws_join + p.workers);
     k.ws_ml = k.ws_o + (size_t)p.workers * p.lanes * 2 * p.tile_rows * HEAD;
@@ -470,7 +486,7 @@ jl_status tree_attention(const jl_tree_attn& a, cudaStream_t st) {
     const bool f = a.dtype == JL_KV_F32;
     if (a.pool.dtype == JL_KV_BF16) JL_TRY(tc_launch(k, f, st));
     else JL_TRY((f ? launch_cc<float>(k, st) : launch_cc<uint16_t>(k, st)));
-    if (p.workers > 1) {
+    if (p.bytes) {
         // all blocks resident, at most one per row there may be
         const long long most = (long long)(p.workers - 1) * a.max_nodes * k.group;
         const dim3 grid((unsigned)std::min<long long>((long long)CB_PER_SM * on.sms, most));

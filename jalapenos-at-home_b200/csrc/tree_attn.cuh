@@ -13,7 +13,8 @@
 // two partials: the item its range starts in (slot 0) and the item its range
 // ends in (slot 1).  The first worker w whose pages start inside an item says
 // in ws_join[w] what there is to add: the partial of worker w - 1 (slot 1) and
-// those of w, w + 1 .. (slot 0).
+// those of w, w + 1 .. (slot 0).  Where no sequence can have more than a few
+// pages (`whole`), an item is one unit: none is split, and nothing is joined.
 //
 // The query rows of an item are node * group + head of the group, cut into
 // tiles of `tile_rows`; a worker is `lanes` CTAs, one per tile, that walk the
@@ -53,6 +54,7 @@ struct Args {
     float* ws_o;       // [worker][lane][slot][tile_rows][HEAD]
     float* ws_ml;      // [worker][lane][slot][tile_rows][2]: maximum (scores times c2), sum
     int workers, lanes, tile_rows, min_units;
+    int whole;         // items are not split
     int q_tma;         // the tensor-core kernel's queries come by TMA
     int32_t* status;
 };
@@ -101,7 +103,8 @@ __device__ __forceinline__ Split split_of(const Args& a, int total) {
     return s;
 }
 
-__device__ __forceinline__ int units_of(const Args& a, const Seq& q) { return q.np ? a.kv_heads * (q.np + SEG) : 0; }
+__device__ __forceinline__ int item_units(const Args& a, const Seq& q) { return a.whole ? 1 : q.np + SEG; }
+__device__ __forceinline__ int units_of(const Args& a, const Seq& q) { return q.np ? a.kv_heads * item_units(a, q) : 0; }
 
 struct Found {     // the sequence a worker's range starts in
     Seq q;
@@ -170,15 +173,15 @@ struct Walk {
         end = to;
         if (from >= end || s >= a.seqs) return false;
         q = f.q;
-        h = (from - f.first) / (q.np + SEG);
-        item = f.first + h * (q.np + SEG);
-        p0 = max(0, from - item - SEG);
-        p1 = min(q.np, end - item - SEG);
+        h = (from - f.first) / item_units(a, q);
+        item = f.first + h * item_units(a, q);
+        p0 = a.whole ? 0 : max(0, from - item - SEG);
+        p1 = a.whole ? q.np : min(q.np, end - item - SEG);
         return p1 > p0 || next(a);
     }
     __device__ bool next(const Args& a) {
-        item += q.np + SEG;
-        if (item + SEG >= end) return false;  // no page of the next item
+        item += item_units(a, q);
+        if (item + (a.whole ? 0 : SEG) >= end) return false;  // no page of the next item
         if (++h >= a.kv_heads) {
             h = 0;
             do {
@@ -187,7 +190,7 @@ struct Walk {
             } while (q.np == 0);
         }
         p0 = 0;
-        p1 = min(q.np, end - item - SEG);
+        p1 = a.whole ? q.np : min(q.np, end - item - SEG);
         return true;
     }
     // Worker w's entry of ws_join, (row of node 0, nodes, KV head, partials), from
@@ -201,9 +204,14 @@ struct Walk {
     __device__ int slot() const { return p0 > 0 ? 0 : 1; }
 };
 
+// The first word of a node's mask, to be on its way before it is needed.
+__device__ __forceinline__ uint64_t first_word(const Args& a, const Seq& q, int node) {
+    return a.mask ? a.mask[(size_t)(q.lo + node) * a.mask_words] : 0;
+}
+
 // The positions of page p that node `node` (row `lo + node`) sees, bit i =
-// position 64 p + i.
-__device__ __forceinline__ uint64_t visible(const Args& a, const Seq& q, int node, int p) {
+// position 64 p + i; m0: its mask's first word.
+__device__ __forceinline__ uint64_t visible(const Args& a, const Seq& q, int node, int p, uint64_t m0) {
     const long long first = (long long)p * PAGE;
     const long long base = first - q.ctx;  // node index of bit 0
     if (base + PAGE <= 0) return ~0ull;    // committed positions only
@@ -212,10 +220,10 @@ __device__ __forceinline__ uint64_t visible(const Args& a, const Seq& q, int nod
         const uint64_t* m = a.mask + (size_t)(q.lo + node) * a.mask_words;
         if (base >= 0) {
             const int w = (int)(base >> 6), sh = (int)(base & 63);
-            v = w < a.mask_words ? m[w] >> sh : 0;
+            v = w == 0 ? m0 >> sh : w < a.mask_words ? m[w] >> sh : 0;
             if (sh && w + 1 < a.mask_words) v |= m[w + 1] << (64 - sh);
         } else {
-            v = (m[0] << (int)-base) | ((1ull << (int)-base) - 1);
+            v = (m0 << (int)-base) | ((1ull << (int)-base) - 1);
         }
         const long long left = q.n - base;  // nodes past the tree are not seen
         if (left < PAGE) v &= (1ull << (int)max(left, 0ll)) - 1;

@@ -242,7 +242,7 @@ __device__ __noinline__ void add_odd(const Args a, const Walk w, int g, bool min
         for (int p = max(w.p0, w.q.ctx / PAGE); mine && p < w.p1; ++p) {
             const int page = pt[p];
             if ((unsigned)page >= (unsigned)a.pages) continue;
-            const uint64_t vis = visible(a, w.q, node, p);
+            const uint64_t vis = visible(a, w.q, node, p, first_word(a, w.q, node));
             for (int r = 0; r < PAGE; ++r) {
                 const long long pos = (long long)p * PAGE + r;
                 if (!(vis >> r & 1) || pos < w.q.ctx) continue;
@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
     Walk w;
     const bool work = w.start(a, ctl.locate.found, sp.at(worker), sp.at(worker + 1)) && !(ptx::smem_u32(sm) & 1023);
     const int row0 = tile * ROWS;
-    if (tid == 0 && tile == 0 && a.workers > 1) a.ws_join[worker] = w.join(sp, worker, work);
+    if (tid == 0 && tile == 0 && a.workers > 1 && !a.whole) a.ws_join[worker] = w.join(sp, worker, work);
 
     if (work && warp == W_TMA && lane == 0) {
         const int none = a.pages * a.kv_heads * PAGE;  // the row after the pool's last
@@ -459,6 +459,7 @@ __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
             float m = -INFINITY, l = 0.f;
             bool odd = false;  // this thread took a value out
             int page = pt[w.p0];
+            const uint64_t m0 = mine ? first_word(a, w.q, node) : 0;
             // Warps that exchange leave the loop together: a wait that gives up
             // only clears ok, until the exchange tells all of them.
             for (int i = 0; i < n; ++i, ++it) {
@@ -497,7 +498,7 @@ __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
                         all_of<32 * SPLIT>(true);  // every part was read
                     }
                     if (edge) {
-                        const uint64_t vis = mine && there ? visible(a, w.q, node, p) : 0;
+                        const uint64_t vis = mine && there ? visible(a, w.q, node, p, m0) : 0;
                         const uint32_t v0 = (uint32_t)vis, v1 = (uint32_t)(vis >> 32);
 #pragma unroll
                         for (int c = 0; c < 32; ++c) {

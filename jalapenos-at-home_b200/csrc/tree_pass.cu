@@ -146,7 +146,7 @@ jl_status record_tree_pass(jl_model* m, const jl_cache* c, const TreeBuffers& t,
     a.mask = &t.dev->mask[0][0];
     a.mask_words = MASK_WORDS;
     a.page_table = c->d_pages;
-    a.max_pages = (int)c->max_pages;
+    a.max_pages = (int)((c->len + n + PAGE - 1) / PAGE);  // one sequence: the table has one row
     a.workspace = t.workspace;
     a.workspace_bytes = t.workspace_bytes;
     a.status = m->counters;
