@@ -1,6 +1,6 @@
 // Attention of the nodes of drafted trees over the paged cache
-// (jl_tree_attention): host checks, the CUDA-core kernel and the kernel that
-// adds the partial results of items that several workers share.
+// (jl_tree_attention): host checks and the kernel that adds the partial results
+// of items that several workers share.  The attention itself: tree_attn_tc.cu.
 #include <algorithm>
 #include <cmath>
 #include <mutex>
@@ -15,187 +15,9 @@ namespace jl {
 namespace tree {
 namespace {
 
-__device__ __forceinline__ float4 load4(const float* p) { return *(const float4*)p; }
-__device__ __forceinline__ float4 load4(const uint16_t* p) {
-    const uint2 w = *(const uint2*)p;
-    return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
-                       __uint_as_float(w.y & 0xffff0000u));
-}
 __device__ __forceinline__ void store4(float* p, float4 v) { *(float4*)p = v; }
 __device__ __forceinline__ void store4(uint16_t* p, float4 v) {
     *(uint2*)p = make_uint2(f2bf16(v.x) | (uint32_t)f2bf16(v.y) << 16, f2bf16(v.z) | (uint32_t)f2bf16(v.w) << 16);
-}
-
-// ---- CUDA cores: pools of f32 pages -----------------------------------------------
-//
-// A CTA holds a tile of 16 * RT query rows and walks its range page by page:
-// K and V of a page go to shared memory as f32; thread (ty, tx) scores keys
-// tx + 16 i of rows ty + 16 j, the 16 threads of a row share its running
-// maximum and sum (online softmax, base 2), and each keeps dims 4 tx .. and
-// 64 + 4 tx .. of the row's output.
-constexpr int CC_T = 256;
-constexpr int CC_KLD = HEAD + 4;  // K rows padded: 8 rows' float4s on all banks
-constexpr int CC_PLD = PAGE + 4;
-
-template <int RT>
-constexpr size_t cc_smem() {
-    return sizeof(float) * ((size_t)16 * RT * CC_KLD + PAGE * CC_KLD + PAGE * HEAD + 16 * RT * CC_PLD);
-}
-
-template <typename T, int RT>
-__global__ void __launch_bounds__(CC_T, RT <= 2 ? 2 : 1) k_tree_attn_cc(Args a) {
-    extern __shared__ __align__(16) float cc_smem_raw[];
-    float* qs = cc_smem_raw;                  // [16 RT][CC_KLD]
-    float* ks = qs + 16 * RT * CC_KLD;        // [PAGE][CC_KLD]
-    float* vs = ks + PAGE * CC_KLD;           // [PAGE][HEAD]
-    float* ps = vs + PAGE * HEAD;             // [16 RT][CC_PLD]
-    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-    const int worker = blockIdx.x, lane = blockIdx.y;
-    constexpr int R = 16 * RT;
-    ptx::grid_dependency_wait();
-    ptx::launch_dependents();
-    __shared__ LocateScratch scratch;
-    const Split sp = locate<CC_T>(a, worker, scratch);
-    Walk w;
-    const bool work = w.start(a, scratch.found, sp.at(worker), sp.at(worker + 1));
-    if (tid == 0 && lane == 0 && a.workers > 1 && !a.whole) a.ws_join[worker] = w.join(sp, worker, work);
-    if (!work) return;
-    do {
-        const int live = min(R, w.q.n * a.group - lane * R);  // rows of this tile
-        if (live <= 0) continue;
-        __syncthreads();  // the previous segment's tiles are no longer read
-        for (int i = tid; i < R * 32; i += CC_T) {
-            const int r = i >> 5, c = i & 31, g = lane * R + r;
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (r < live)
-                v = load4((const T*)a.q + (size_t)(w.q.lo + g / a.group) * a.q_ld +
-                          (size_t)(w.h * a.group + g % a.group) * HEAD + 4 * c);
-            *(float4*)(qs + r * CC_KLD + 4 * c) = v;
-        }
-        float m[RT], l[RT], acc[RT][8];
-        uint64_t m0[RT];
-#pragma unroll
-        for (int j = 0; j < RT; ++j) {
-            m[j] = -INFINITY;
-            l[j] = 0.f;
-            m0[j] = ty + 16 * j < live ? first_word(a, w.q, (lane * R + ty + 16 * j) / a.group) : 0;
-#pragma unroll
-            for (int d = 0; d < 8; ++d) acc[j][d] = 0.f;
-        }
-        const int32_t* pt = a.page_table + (size_t)w.s * a.max_pages;
-        for (int p = w.p0; p < w.p1; ++p) {
-            const int page = pt[p];
-            const bool there = (unsigned)page < (unsigned)a.pages;
-            if (!there && tid == 0) flag(a.status, ST_PAGE);
-            const int used = there ? (int)min((long long)PAGE, (long long)w.q.ctx + w.q.n - (long long)p * PAGE) : 0;
-            __syncthreads();  // the previous page's tiles are no longer read
-            const size_t at = kv_index(there ? page : 0, w.h, 0, a.kv_heads);
-            constexpr int LOADS = PAGE * 32 / CC_T;
-            float4 kk[LOADS], vv[LOADS];  // all in flight
-#pragma unroll
-            for (int i = 0; i < LOADS; ++i) {
-                const int r = (tid + i * CC_T) >> 5, c = tid & 31;
-                kk[i] = vv[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (r < used) {  // rows past the sequence may hold anything
-                    kk[i] = load4((const float*)a.k + at + (size_t)r * HEAD + 4 * c);
-                    vv[i] = load4((const float*)a.v + at + (size_t)r * HEAD + 4 * c);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < LOADS; ++i) {
-                const int r = (tid + i * CC_T) >> 5, c = tid & 31;
-                *(float4*)(ks + r * CC_KLD + 4 * c) = kk[i];
-                *(float4*)(vs + r * HEAD + 4 * c) = vv[i];
-            }
-            __syncthreads();
-            const bool edge = (long long)(p + 1) * PAGE > w.q.ctx || !there;
-            uint64_t vis[RT];
-#pragma unroll
-            for (int j = 0; j < RT; ++j) {
-                const int r = ty + 16 * j;
-                vis[j] = 0;
-                if (16 * j + (ty & ~1) >= live) break;  // neither row of the warp is live
-                vis[j] = !there || r >= live ? 0 : edge ? visible(a, w.q, (lane * R + r) / a.group, p, m0[j]) : ~0ull;
-                float sc[4] = {0.f, 0.f, 0.f, 0.f};
-                const float* qr = qs + r * CC_KLD;
-#pragma unroll 8
-                for (int c = 0; c < 32; ++c) {
-                    const float4 q4 = *(const float4*)(qr + 4 * c);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float4 k4 = *(const float4*)(ks + (tx + 16 * i) * CC_KLD + 4 * c);
-                        sc[i] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, sc[i]))));
-                    }
-                }
-                float top = m[j];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    sc[i] = vis[j] >> (tx + 16 * i) & 1 ? __fmul_rn(sc[i], a.c2) : -INFINITY;
-                    top = fmaxf(top, sc[i]);
-                }
-#pragma unroll
-                for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                const float ref = top == -INFINITY ? 0.f : top;
-                const float corr = ex2(m[j] - ref);  // 0 while nothing was seen
-                float sum = 0.f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float e = vis[j] >> (tx + 16 * i) & 1 ? ex2(sc[i] - ref) : 0.f;
-                    ps[r * CC_PLD + tx + 16 * i] = e;
-                    sum += e;
-                }
-#pragma unroll
-                for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                l[j] = fmaf(l[j], corr, sum);
-                m[j] = top;
-#pragma unroll
-                for (int d = 0; d < 8; ++d) acc[j][d] *= corr;
-            }
-            __syncwarp();  // a row's weights are read by the half warp that wrote them
-            for (int key = 0; key < PAGE; ++key) {
-                const float4 v0 = *(const float4*)(vs + key * HEAD + 4 * tx);
-                const float4 v1 = *(const float4*)(vs + key * HEAD + 64 + 4 * tx);
-#pragma unroll
-                for (int j = 0; j < RT; ++j) {
-                    if (16 * j + (ty & ~1) >= live) break;
-                    // not seen: skipped, not multiplied by zero (V may be infinite)
-                    if (edge && !(vis[j] >> key & 1)) continue;
-                    const float e = ps[(ty + 16 * j) * CC_PLD + key];
-                    acc[j][0] = fmaf(e, v0.x, acc[j][0]);
-                    acc[j][1] = fmaf(e, v0.y, acc[j][1]);
-                    acc[j][2] = fmaf(e, v0.z, acc[j][2]);
-                    acc[j][3] = fmaf(e, v0.w, acc[j][3]);
-                    acc[j][4] = fmaf(e, v1.x, acc[j][4]);
-                    acc[j][5] = fmaf(e, v1.y, acc[j][5]);
-                    acc[j][6] = fmaf(e, v1.z, acc[j][6]);
-                    acc[j][7] = fmaf(e, v1.w, acc[j][7]);
-                }
-            }
-        }
-        const bool whole = w.whole();
-        const size_t part = (((size_t)worker * a.lanes + lane) * 2 + w.slot()) * R;
-#pragma unroll
-        for (int j = 0; j < RT; ++j) {
-            const int r = ty + 16 * j, g = lane * R + r;
-            if (r >= live) continue;
-            float4 o0 = make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
-            float4 o1 = make_float4(acc[j][4], acc[j][5], acc[j][6], acc[j][7]);
-            if (whole) {
-                const float inv = l[j] == 0.f ? 0.f : __fdiv_rn(1.f, l[j]);  // 0: nothing seen
-                const int row = w.q.lo + g / a.group, head = w.h * a.group + g % a.group;
-                T* dst = (T*)a.out + (size_t)row * a.out_ld + (size_t)head * HEAD;
-                store4(dst + 4 * tx, make_float4(o0.x * inv, o0.y * inv, o0.z * inv, o0.w * inv));
-                store4(dst + 64 + 4 * tx, make_float4(o1.x * inv, o1.y * inv, o1.z * inv, o1.w * inv));
-                if (a.lse && tx == 0)
-                    a.lse[(size_t)row * a.q_heads + head] =
-                        l[j] == 0.f ? -INFINITY : (m[j] + log2f(l[j])) * LN2;
-            } else {
-                store4(a.ws_o + (part + r) * HEAD + 4 * tx, o0);
-                store4(a.ws_o + (part + r) * HEAD + 64 + 4 * tx, o1);
-                if (tx == 0) *(float2*)(a.ws_ml + (part + r) * 2) = make_float2(m[j], l[j]);
-            }
-        }
-    } while (w.next(a));
 }
 
 // ---- partial results -----------------------------------------------------------------
@@ -365,18 +187,18 @@ struct Plan {
 Plan plan_of(const jl_tree_attn& a, int sms) {
     Plan p;
     const int rows = a.max_nodes * (a.q_heads / a.pool.kv_heads);
-    const bool tc = a.pool.dtype == JL_KV_BF16;
-    p.tile_rows = tc ? tc_tile_rows(a.dtype == JL_KV_F32) : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+    const bool rows_f32 = a.dtype == JL_KV_F32, pool_f32 = a.pool.dtype == JL_KV_F32;
+    p.tile_rows = tc_tile_rows(rows_f32, pool_f32);
     p.lanes = (rows + p.tile_rows - 1) / p.tile_rows;
-    p.workers = std::min(CB_MOST, std::max(1, (tc ? TC_CTAS_PER_SM : p.tile_rows <= 32 ? 2 : 1) * sms / p.lanes));
+    p.workers = std::min(CB_MOST, std::max(1, tc_ctas(pool_f32) * sms / p.lanes));
     // Whole items or split ones: whole, a worker's longest item sets the time (in
     // waves of all workers); split, the mean does, and the join is added.  The
-    // times, in us on a B200 with every SM busy, are a page's (tensor cores: 1.5
-    // for bf16 rows, 2 for f32; CUDA cores: 8), a segment's start and end (6) and
+    // times, in us on a B200 with every SM busy, are a page's (1.5 for bf16
+    // rows and pools, 2 with f32), a segment's start and end (6) and
     // the join (5).  Measured whole / split, 8 bf16 nodes, 32 heads over 8: one
     // sequence of 300 positions 10.6 / 14.7 us, 32 of them 15.3 / 30.4 us, 32 of up
     // to 700 23.6 / 34.5 us; f32 rows, one sequence of 700 29.6 / 20.9 us.
-    const double page = !tc ? 8.0 : a.dtype == JL_KV_F32 ? 2.0 : 1.5;
+    const double page = rows_f32 || pool_f32 ? 2.0 : 1.5;
     const double ctas = (double)a.seqs * a.pool.kv_heads * p.lanes, slots = (double)p.workers * p.lanes;
     const double whole = std::ceil(ctas / slots) * (a.max_pages * page + 6);
     const double split = std::max(ctas * (a.max_pages + SEG) / slots, 1.0 + SEG) * page + 6 + 5;
@@ -387,29 +209,11 @@ Plan plan_of(const jl_tree_attn& a, int sms) {
     return p;
 }
 
-template <typename T>
-jl_status launch_cc(const Args& a, cudaStream_t st) {
-    const dim3 grid(a.workers, a.lanes);
-    if (a.tile_rows == 16) return launch_pdl(k_tree_attn_cc<T, 1>, grid, dim3(CC_T), cc_smem<1>(), st, a);
-    if (a.tile_rows == 32) return launch_pdl(k_tree_attn_cc<T, 2>, grid, dim3(CC_T), cc_smem<2>(), st, a);
-    return launch_pdl(k_tree_attn_cc<T, 4>, grid, dim3(CC_T), cc_smem<4>(), st, a);
-}
-
-template <typename T>
-jl_status configure_cc() {
-    JL_CUDA(cudaFuncSetAttribute(k_tree_attn_cc<T, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cc_smem<1>()));
-    JL_CUDA(cudaFuncSetAttribute(k_tree_attn_cc<T, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cc_smem<2>()));
-    JL_CUDA(cudaFuncSetAttribute(k_tree_attn_cc<T, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cc_smem<4>()));
-    return JL_OK;
-}
-
 jl_status configure(int device) {  // once per device
     static std::mutex mu;
     static bool done[64] = {};
     std::lock_guard<std::mutex> g(mu);
     if (device < 64 && done[device]) return JL_OK;
-    JL_TRY((configure_cc<float>()));
-    JL_TRY((configure_cc<uint16_t>()));
     JL_TRY(tc_configure());
     if (device < 64) done[device] = true;
     return JL_OK;
@@ -484,8 +288,7 @@ jl_status tree_attention(const jl_tree_attn& a, cudaStream_t st) {
     k.ws_ml = k.ws_o + (size_t)p.workers * p.lanes * 2 * p.tile_rows * HEAD;
     k.status = a.status;
     const bool f = a.dtype == JL_KV_F32;
-    if (a.pool.dtype == JL_KV_BF16) JL_TRY(tc_launch(k, f, st));
-    else JL_TRY((f ? launch_cc<float>(k, st) : launch_cc<uint16_t>(k, st)));
+    JL_TRY(tc_launch(k, f, a.pool.dtype == JL_KV_F32, st));
     if (p.bytes) {
         // all blocks resident, at most one per row there may be
         const long long most = (long long)(p.workers - 1) * a.max_nodes * k.group;

@@ -247,12 +247,12 @@ __device__ __forceinline__ int div_small(int i, float inv) { return (int)(((floa
 
 constexpr float LN2 = 0.6931471805599453f;
 
-// Tensor-core kernel (tree_attn_tc.cu): query rows of a tile, CTAs per SM, and
-// the launch over a pool of bf16 pages; `f32`: the type of the q and out rows.
-constexpr int TC_CTAS_PER_SM = 2;
-constexpr int tc_tile_rows(bool f32) { return f32 ? 32 : 128; }
+// The attention kernel (tree_attn_tc.cu): query rows of a tile, CTAs per SM, and
+// the launch, by the types of the rows (q and out) and of the pool.
+constexpr int tc_tile_rows(bool rows_f32, bool pool_f32) { return rows_f32 || pool_f32 ? 32 : 128; }
+constexpr int tc_ctas(bool pool_f32) { return pool_f32 ? 1 : 2; }
 jl_status tc_configure();
-jl_status tc_launch(Args a, bool f32, cudaStream_t st);
+jl_status tc_launch(Args a, bool rows_f32, bool pool_f32, cudaStream_t st);
 
 }  // namespace tree
 }  // namespace jl

@@ -1,4 +1,4 @@
-// Tree attention on tensor cores, for pools of bf16 pages.
+// Tree attention on tensor cores.
 //
 // A CTA walks its worker's range (tree_attn.cuh) page by page with six warps:
 // warp 5 brings K and V pages into two rings by TMA, warp 4 issues the MMAs,
@@ -26,6 +26,12 @@
 // a value get it added from global memory at the end.
 // A page outside the pool is read as rows past the end of the tensor map,
 // which arrive as zeros, and masked.
+//
+// Pools of f32 pages: eight warps take the place of the TMA warp.  They load a
+// head's K or V rows into registers, two pages' worth ahead, and write them to
+// the rings as three bf16 pieces by truncation (24 bits, exact), so S and O take
+// three MMA groups a page; the rows are stacked as above whatever their type,
+// and one CTA fills an SM.  Clearing V happens on the way.
 #include <cuda.h>
 #include <cuda_bf16.h>
 
@@ -41,45 +47,49 @@ namespace {
 
 using mx::swz128;
 
-constexpr int T_THREADS = 192;
-constexpr int W_MMA = 4, W_TMA = 5;
+constexpr int W_MMA = 4, W_LOAD = 5;
 constexpr uint32_t PAGE_BYTES = PAGE * HEAD * 2;  // one head's K or V of a page: two boxes of 64 dims
 constexpr uint32_t BOX_BYTES = PAGE_BYTES / 2;
 constexpr uint32_t COL_O = 128, TMEM_COLS = 256;
 constexpr uint32_t WAIT_POLLS = 1u << 20;
 constexpr float MOVE = 8.f;  // log2 of how far a row's maximum may grow before it is moved
 
-// NP: pieces of the weights in a row's columns.  SPLIT: warps that hold the
-// pieces of the same rows.
-template <typename T>
-struct Cfg;
-template <>
-struct Cfg<uint16_t> {
-    static constexpr int ROWS = tc_tile_rows(false), NP = 2, SPLIT = 1, NK = 3, NV = 2, Q_ROWS = 128, XCH = 0;
+// T: type of the rows, KV: of the pool.  SPLIT: warps that hold the pieces of the
+// same rows.  NP: pieces of the weights in a row's columns.  KVP: pieces of a
+// page.  LOADERS: warps that bring the pages.
+template <typename T, typename KV>
+struct Cfg {
+    static constexpr bool ROWS_F32 = sizeof(T) == 4, POOL_F32 = sizeof(KV) == 4;
+    static constexpr int SPLIT = ROWS_F32 || POOL_F32 ? 3 : 1, NP = SPLIT > 1 ? 1 : 2, KVP = POOL_F32 ? 3 : 1;
+    static constexpr int ROWS = tc_tile_rows(ROWS_F32, POOL_F32), Q_ROWS = SPLIT > 1 ? SPLIT * ROWS : 128;
+    static constexpr int NK = SPLIT > 1 ? 2 : 3, NV = POOL_F32 ? 1 : 2;
+    static constexpr int XCH = SPLIT > 1 ? SPLIT * ROWS * 64 * 4 : 0;  // the exchange: 64 floats of every row and part
+    static constexpr int LOADERS = POOL_F32 ? 8 : 1, THREADS = 32 * (5 + LOADERS), CTAS = tc_ctas(POOL_F32);
+    static constexpr uint32_t SLOT = KVP * PAGE_BYTES;
 };
-template <>
-struct Cfg<float> {
-    static constexpr int ROWS = tc_tile_rows(true), NP = 1, SPLIT = 3, NK = 2, NV = 2, Q_ROWS = SPLIT * ROWS;
-    static constexpr int XCH = SPLIT * ROWS * 64 * 4;  // the exchange: 64 floats of every row and part
-};
+static_assert(Cfg<float, float>::ROWS == 32 && Cfg<uint16_t, uint16_t>::ROWS == 128, "tiles");
 constexpr int SB = 2;  // S buffers
 
-template <int NK, int NV>
+template <typename C>
 struct Ctl {
-    uint64_t kfull[NK], kempty[NK], vfull[NV], vempty[NV];
+    uint64_t kfull[C::NK], kempty[C::NK], vfull[C::NV], vempty[C::NV];
     uint64_t sfull[2], pfull[2], odone[2];  // by page parity
     uint64_t qfull, ofree, drain;
     uint32_t tmem;
-    int stop;  // a wait gave up: every role leaves
+    int stop;    // a wait gave up: every role leaves
+    // The loader warps of an f32 pool took a value out of segment s: odd[s % 4] is
+    // s + 1 (they are less than four segments ahead: the rings hold three pages)
+    int odd[4];
     LocateScratch locate;
 };
 
-template <typename T>
-constexpr uint32_t q_bytes() { return Cfg<T>::Q_ROWS * HEAD * 2; }
-template <typename T>
-constexpr size_t tc_smem() { return q_bytes<T>() + (size_t)(Cfg<T>::NK + Cfg<T>::NV) * PAGE_BYTES + Cfg<T>::XCH + 1024; }
-static_assert(tc_smem<float>() <= 113 * 1024 && tc_smem<uint16_t>() <= 113 * 1024, "two CTAs an SM");
-static_assert(sizeof(Ctl<3, 2>) <= 1024, "control block");
+template <typename C>
+constexpr uint32_t q_bytes() { return C::Q_ROWS * HEAD * 2; }
+template <typename C>
+constexpr size_t tc_smem() { return q_bytes<C>() + (size_t)(C::NK + C::NV) * C::SLOT + C::XCH + 1024; }
+static_assert(sizeof(Ctl<Cfg<uint16_t, uint16_t>>) <= 1024, "control block");
+static_assert(tc_smem<Cfg<float, uint16_t>>() <= 113 * 1024 && tc_smem<Cfg<uint16_t, uint16_t>>() <= 113 * 1024, "two CTAs an SM");
+static_assert(tc_smem<Cfg<float, float>>() <= 227 * 1024, "one CTA an SM");
 
 // Waits for a phase, for WAIT_POLLS polls or until another role stops.
 __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volatile int* stop) {
@@ -118,35 +128,40 @@ __device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
 __device__ __forceinline__ float lo_f(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float hi_f(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
-// Query rows of a tile into shared memory as bf16 pieces, by the 128 softmax
-// threads: [64-dim block][lane][128 B], swizzled.  bf16 rows of groups that
+// Query rows of a tile into shared memory, by the 128 softmax threads:
+// [64-dim block][lane][128 B], swizzled.  Unstacked bf16 rows of groups that
 // divide the tile come by TMA instead.
-__device__ __forceinline__ void load_q(const Args& a, const Walk& w, int row0, int live, float inv_group, uint8_t* sm, int tid,
-                                       const uint16_t*) {
-    constexpr int R = Cfg<uint16_t>::ROWS;
-    const uint16_t* q = (const uint16_t*)a.q + (size_t)w.q.lo * a.q_ld + (size_t)w.h * a.group * HEAD;
+template <typename C, typename T>
+__device__ __forceinline__ void load_q(const Args& a, const Walk& w, int row0, int live, float inv_group, uint8_t* sm, int tid) {
+    const T* q = (const T*)a.q + (size_t)w.q.lo * a.q_ld + (size_t)w.h * a.group * HEAD;
+    auto row = [&](int r) {
+        const int node = div_small(row0 + r, inv_group);
+        return q + node * a.q_ld + (row0 + r - node * a.group) * HEAD;
+    };
+    if constexpr (C::SPLIT == 1) {
 #pragma unroll 8
-    for (int i = tid; i < live * 16; i += 128) {
-        const int r = i >> 4, c = i & 15, node = div_small(row0 + r, inv_group), h = row0 + r - node * a.group;
-        const uint4 v = *(const uint4*)(q + node * a.q_ld + h * HEAD + 8 * c);
-        *(uint4*)(sm + (c >> 3) * (R * 128) + swz128((uint32_t)r, (uint32_t)(c & 7) * 16)) = v;
-    }
-}
-__device__ __forceinline__ void load_q(const Args& a, const Walk& w, int row0, int live, float inv_group, uint8_t* sm, int tid,
-                                       const float*) {
-    constexpr int R = Cfg<float>::ROWS, Q = Cfg<float>::Q_ROWS;
-    const float* q = (const float*)a.q + (size_t)w.q.lo * a.q_ld + (size_t)w.h * a.group * HEAD;
+        for (int i = tid; i < live * 16; i += 128) {
+            const int r = i >> 4, c = i & 15;
+            *(uint4*)(sm + (c >> 3) * (C::Q_ROWS * 128) + swz128((uint32_t)r, (uint32_t)(c & 7) * 16)) = *(const uint4*)(row(r) + 8 * c);
+        }
+    } else {
 #pragma unroll
-    for (int i = tid; i < R * 32; i += 128) {
-        const int r = i >> 5, c = i & 31;
-        if (r >= live) break;
-        const int node = div_small(row0 + r, inv_group), h = row0 + r - node * a.group;
-        float4 v = *(const float4*)(q + node * a.q_ld + h * HEAD + 4 * c);
+        for (int i = tid; i < C::ROWS * 32; i += 128) {
+            const int r = i >> 5, c = i & 31;
+            if (r >= live) break;
+            float4 v;
+            if constexpr (sizeof(T) == 4) {
+                v = *(const float4*)(row(r) + 4 * c);
+            } else {
+                const uint2 u = *(const uint2*)(row(r) + 4 * c);
+                v = make_float4(lo_f(u.x), hi_f(u.x), lo_f(u.y), hi_f(u.y));
+            }
 #pragma unroll
-        for (int p = 0; p < 3; ++p) {  // lanes 32 p + r
-            const uint32_t x = pack_bf16(v.x, v.y), y = pack_bf16(v.z, v.w);
-            *(uint2*)(sm + (c >> 4) * (Q * 128) + swz128((uint32_t)(p * R + r), (uint32_t)(c & 15) * 8)) = make_uint2(x, y);
-            v = make_float4(v.x - lo_f(x), v.y - hi_f(x), v.z - lo_f(y), v.w - hi_f(y));
+            for (int p = 0; p < C::SPLIT; ++p) {  // lanes ROWS p + r
+                const uint32_t x = pack_bf16(v.x, v.y), y = pack_bf16(v.z, v.w);
+                *(uint2*)(sm + (c >> 4) * (C::Q_ROWS * 128) + swz128((uint32_t)(p * C::ROWS + r), (uint32_t)(c & 15) * 8)) = make_uint2(x, y);
+                v = make_float4(v.x - lo_f(x), v.y - hi_f(x), v.z - lo_f(y), v.w - hi_f(y));
+            }
         }
     }
 }
@@ -159,16 +174,18 @@ constexpr uint32_t DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
 __device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo) { return (saddr >> 4) | ((lbo >> 4) << 16); }
 __device__ __forceinline__ uint64_t desc(uint32_t lo) { return (uint64_t)DESC_HI << 32 | lo; }
 
-// S = Q K^T of one page; q, k: low words.
-template <typename T>
+// S = Q K^T of one page, its pieces smallest first; q, k: low words.
+template <typename C>
 __device__ __forceinline__ void issue_scores(uint32_t q, uint32_t k, uint32_t tmem_s) {
     const uint32_t idesc = ptx::bf16_idesc(128, PAGE);
 #pragma unroll
-    for (int db = 0; db < 2; ++db)
+    for (int p = C::KVP - 1; p >= 0; --p)
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
-            ptx::mma_bf16(tmem_s, desc(q + ((db * Cfg<T>::Q_ROWS * 128 + 32 * s) >> 4)), desc(k + ((db * BOX_BYTES + 32 * s) >> 4)),
-                          idesc, (db || s) ? 1u : 0u);
+        for (int db = 0; db < 2; ++db)
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                ptx::mma_bf16(tmem_s, desc(q + ((db * C::Q_ROWS * 128 + 32 * s) >> 4)),
+                              desc(k + ((p * PAGE_BYTES + db * BOX_BYTES + 32 * s) >> 4)), idesc, (p < C::KVP - 1 || db || s) ? 1u : 0u);
 }
 
 // The exchange between the warps that hold the pieces of 32 f32 rows: floats
@@ -184,15 +201,17 @@ __device__ __forceinline__ float4 xch_sum(uint8_t* xch, int row, int c) {
 
 // O += P V of one page: P from TMEM, V (low word v) as an MN-major operand
 // (64-dim blocks BOX_BYTES apart, groups of 8 keys 1024 bytes apart).
-template <typename T>
+template <typename C>
 __device__ __forceinline__ void issue_pv(uint32_t tmem_p, uint32_t v, uint32_t tmem_o, bool first) {
     const uint32_t idesc = ptx::bf16_idesc(128, HEAD) | (1u << 16);
 #pragma unroll
-    for (int p = Cfg<T>::NP - 1; p >= 0; --p)
+    for (int vp = C::KVP - 1; vp >= 0; --vp)
 #pragma unroll
-        for (int s = 0; s < 4; ++s)  // keys 16 s ..
-            ptx::mma_bf16_ta(tmem_o, tmem_p + 32 * p + 8 * s, desc(v + (2048 * s >> 4)), idesc,
-                             (p < Cfg<T>::NP - 1 || s || !first) ? 1u : 0u);
+        for (int p = C::NP - 1; p >= 0; --p)
+#pragma unroll
+            for (int s = 0; s < 4; ++s)  // keys 16 s ..
+                ptx::mma_bf16_ta(tmem_o, tmem_p + 32 * p + 8 * s, desc(v + ((vp * PAGE_BYTES + 2048 * s) >> 4)), idesc,
+                                 (vp < C::KVP - 1 || p < C::NP - 1 || s || !first) ? 1u : 0u);
 }
 
 __device__ __forceinline__ bool odd_bf16(uint32_t h) { return (h & 0x7f80u) == 0x7f80u; }  // infinite or NaN
@@ -229,7 +248,9 @@ __device__ __forceinline__ bool clean_v(uint8_t* v, int tree_row, int used, int 
 // Adds what clean_v took out to a warp's rows of O: for every node of this
 // segment's pages that a row sees, its weight times the values that are not
 // finite.  Arguments by value: nothing of the caller's moves to the stack.
-template <typename T>
+__device__ __forceinline__ float value(uint16_t h) { return bf16f(h); }
+__device__ __forceinline__ float value(float f) { return f; }
+template <typename T, typename KV>
 __device__ __noinline__ void add_odd(const Args a, const Walk w, int g, bool mine, float m, uint32_t t_o) {
     const int32_t* pt = a.page_table + (size_t)w.s * a.max_pages;
     const int node = g / a.group;
@@ -246,21 +267,18 @@ __device__ __noinline__ void add_odd(const Args a, const Walk w, int g, bool min
             for (int r = 0; r < PAGE; ++r) {
                 const long long pos = (long long)p * PAGE + r;
                 if (!(vis >> r & 1) || pos < w.q.ctx) continue;
-                const uint16_t* k = (const uint16_t*)a.k + kv_index(page, w.h, r, a.kv_heads);
-                const uint16_t* v = (const uint16_t*)a.v + kv_index(page, w.h, r, a.kv_heads) + d0;
+                const KV* k = (const KV*)a.k + kv_index(page, w.h, r, a.kv_heads);
+                const KV* v = (const KV*)a.v + kv_index(page, w.h, r, a.kv_heads) + d0;
                 float weight = -1.f;
 #pragma unroll
                 for (int d = 0; d < 32; ++d) {
-                    if (!odd_bf16(v[d])) continue;
+                    if (isfinite(value(v[d]))) continue;
                     if (weight < 0.f) {
                         float s = 0.f;
-                        for (int e = 0; e < HEAD; ++e) {
-                            const float x = sizeof(T) == 4 ? ((const float*)q)[e] : bf16f(((const uint16_t*)q)[e]);
-                            s = fmaf(x, bf16f(k[e]), s);
-                        }
+                        for (int e = 0; e < HEAD; ++e) s = fmaf(value(q[e]), value(k[e]), s);
                         weight = ex2(fmaf(s, a.c2, -m));
                     }
-                    o[d] += weight * bf16f(v[d]);
+                    o[d] += weight * value(v[d]);
                 }
             }
         }
@@ -270,6 +288,61 @@ __device__ __noinline__ void add_odd(const Args a, const Walk w, int g, bool min
         ptx::tmem_st32(t_o + d0, bits);
     }
     ptx::tmem_wait_st();
+}
+
+// The loader warps of an f32 pool.  A segment's items, in the order in which the
+// MMAs take them: K 0, K 1, V 0, K 2, V 1, .., V n - 1.
+struct Item {
+    uint32_t it;  // page count of the CTA, for the rings
+    int seg;      // segment count of the CTA
+    bool is_v;
+    int used, tree_row;  // rows of the sequence; those from tree_row on are tree nodes
+};
+struct Items {
+    Walk w;
+    uint32_t it0 = 0;
+    int seg = 0, step = 0;
+    bool more;
+    __device__ bool skip(const Args& a, int row0) const { return w.q.n * a.group <= row0; }
+    __device__ void start(const Args& a, const Walk& from, int row0) {
+        w = from;
+        more = true;
+        while (more && skip(a, row0)) more = w.next(a);
+    }
+    // Loads the next item's rows cw, cw + 8, .. of a warp (lane: 16 bytes of each).
+    __device__ Item fetch(const Args& a, int row0, int cw, int lane, float4 (&x)[PAGE / 8]) {
+        const int n = w.p1 - w.p0;
+        const bool is_v = step >= 2 * n - 1 || (step && step % 2 == 0);
+        const int j = !is_v ? (step + 1) / 2 : step == 2 * n - 1 ? n - 1 : step / 2 - 1, p = w.p0 + j;
+        const int page = a.page_table[(size_t)w.s * a.max_pages + p];
+        const bool there = (unsigned)page < (unsigned)a.pages;
+        if (!there && !is_v && cw == 0 && lane == 0) flag(a.status, ST_PAGE);
+        Item i{it0 + j, seg, is_v, there ? w.q.ctx + w.q.n - p * PAGE : 0, max(0, w.q.ctx - p * PAGE)};
+        const float* src = (const float*)(is_v ? a.v : a.k) + kv_index(there ? page : 0, w.h, 0, a.kv_heads) + 4 * lane;
+#pragma unroll
+        for (int k = 0; k < PAGE / 8; ++k) {
+            const int r = cw + 8 * k;
+            x[k] = r < i.used ? *(const float4*)(src + (size_t)r * HEAD) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        if (++step == 2 * n) {
+            it0 += n;
+            step = 0;
+            ++seg;
+            do more = w.next(a);
+            while (more && skip(a, row0));
+        }
+        return i;
+    }
+};
+
+// One float4 of a row as three pieces by truncation, each the next 8 bits.
+__device__ __forceinline__ void store_pieces(uint8_t* dst, float4 x) {
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+        const uint32_t u0 = __float_as_uint(x.x), u1 = __float_as_uint(x.y), u2 = __float_as_uint(x.z), u3 = __float_as_uint(x.w);
+        *(uint2*)(dst + p * PAGE_BYTES) = make_uint2(__byte_perm(u0, u1, 0x7632), __byte_perm(u2, u3, 0x7632));
+        x = make_float4(x.x - hi_f(u0), x.y - hi_f(u1), x.z - hi_f(u2), x.w - hi_f(u3));
+    }
 }
 
 // A barrier of the first N softmax threads that tells whether `ok` holds for all.
@@ -303,26 +376,27 @@ __device__ __forceinline__ void store_row32<uint16_t>(uint16_t* dst, const float
                                         pack_bf16(o[i + 4] * f, o[i + 5] * f), pack_bf16(o[i + 6] * f, o[i + 7] * f));
 }
 
-template <typename T>
-__global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
+template <typename T, typename KV>
+__global__ void __launch_bounds__(Cfg<T, KV>::THREADS, Cfg<T, KV>::CTAS)
     k_tree_attn_tc(Args a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                    const __grid_constant__ CUtensorMap qmap) {
-    constexpr int ROWS = Cfg<T>::ROWS, NK = Cfg<T>::NK, NV = Cfg<T>::NV, NP = Cfg<T>::NP, SPLIT = Cfg<T>::SPLIT;
+    using C = Cfg<T, KV>;
+    constexpr int ROWS = C::ROWS, NK = C::NK, NV = C::NV, NP = C::NP, SPLIT = C::SPLIT;
     extern __shared__ __align__(1024) uint8_t sm[];
-    uint8_t* kring = sm + q_bytes<T>();
-    uint8_t* vring = kring + NK * PAGE_BYTES;
-    uint8_t* xch = vring + NV * PAGE_BYTES;
-    Ctl<NK, NV>& ctl = *(Ctl<NK, NV>*)(vring + NV * PAGE_BYTES + Cfg<T>::XCH);
+    uint8_t* kring = sm + q_bytes<C>();
+    uint8_t* vring = kring + NK * C::SLOT;
+    uint8_t* xch = vring + NV * C::SLOT;
+    Ctl<C>& ctl = *(Ctl<C>*)(xch + C::XCH);
     volatile int* stop = &ctl.stop;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int worker = blockIdx.x, tile = blockIdx.y;
     if (tid == 0) {
         for (int i = 0; i < NK; ++i) {
-            ptx::mbar_init(&ctl.kfull[i], 1);
+            ptx::mbar_init(&ctl.kfull[i], C::LOADERS);
             ptx::mbar_init(&ctl.kempty[i], 1);
         }
         for (int i = 0; i < NV; ++i) {
-            ptx::mbar_init(&ctl.vfull[i], 1);
+            ptx::mbar_init(&ctl.vfull[i], C::LOADERS);
             ptx::mbar_init(&ctl.vempty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -335,8 +409,11 @@ __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
         ptx::mbar_init(&ctl.drain, 1);
         ptx::fence_barrier_init();
         ctl.stop = 0;
-        ptx::prefetch_tensormap(&kmap);
-        ptx::prefetch_tensormap(&vmap);
+        for (int i = 0; i < 4; ++i) ctl.odd[i] = 0;
+        if (!C::POOL_F32) {
+            ptx::prefetch_tensormap(&kmap);
+            ptx::prefetch_tensormap(&vmap);
+        }
         if (a.q_tma) ptx::prefetch_tensormap(&qmap);
     }
     if (warp == W_MMA) {
@@ -349,13 +426,51 @@ __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
     const uint32_t tmem = ctl.tmem;
     ptx::grid_dependency_wait();
     ptx::launch_dependents();
-    const Split sp = locate<T_THREADS>(a, worker, ctl.locate);
+    const Split sp = locate<C::THREADS>(a, worker, ctl.locate);
     Walk w;
     const bool work = w.start(a, ctl.locate.found, sp.at(worker), sp.at(worker + 1)) && !(ptx::smem_u32(sm) & 1023);
     const int row0 = tile * ROWS;
     if (tid == 0 && tile == 0 && a.workers > 1 && !a.whole) a.ws_join[worker] = w.join(sp, worker, work);
 
-    if (work && warp == W_TMA && lane == 0) {
+    if (C::POOL_F32 && work && warp >= W_LOAD) {
+        const int cw = warp - W_LOAD;
+        Items items;
+        items.start(a, w, row0);
+        float4 x[2][PAGE / 8];  // two items on their way
+        Item at[2];
+        bool have[2] = {false, false}, ok = true;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+            if ((have[b] = items.more)) at[b] = items.fetch(a, row0, cw, lane, x[b]);
+        while (ok && have[0]) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                if (!ok || !have[b]) break;
+                const Item& i = at[b];
+                const uint32_t slot = i.is_v ? i.it % NV : i.it % NK, round = i.is_v ? i.it / NV : i.it / NK;
+                ok = wait_phase(i.is_v ? &ctl.vempty[slot] : &ctl.kempty[slot], (round + 1) & 1, stop);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                uint8_t* dst = (i.is_v ? vring : kring) + slot * C::SLOT + (lane >> 4) * BOX_BYTES;
+                bool odd = false;
+#pragma unroll
+                for (int k = 0; k < PAGE / 8; ++k) {
+                    const int r = cw + 8 * k;
+                    float4 v = x[b][k];
+                    if (i.is_v && r >= i.tree_row && !(isfinite(v.x) && isfinite(v.y) && isfinite(v.z) && isfinite(v.w))) {
+                        odd = true;
+                        v = make_float4(isfinite(v.x) ? v.x : 0.f, isfinite(v.y) ? v.y : 0.f, isfinite(v.z) ? v.z : 0.f, isfinite(v.w) ? v.w : 0.f);
+                    }
+                    store_pieces(dst + swz128((uint32_t)r, (uint32_t)(lane & 15) * 8), v);
+                }
+                if (odd) *(volatile int*)&ctl.odd[i.seg & 3] = i.seg + 1;
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(i.is_v ? &ctl.vfull[slot] : &ctl.kfull[slot]);
+                if ((have[b] = items.more)) at[b] = items.fetch(a, row0, cw, lane, x[b]);
+            }
+        }
+    } else if (!C::POOL_F32 && work && warp == W_LOAD && lane == 0) {
         const int none = a.pages * a.kv_heads * PAGE;  // the row after the pool's last
         uint32_t it = 0, seg = 0;
         bool ok = true;
@@ -411,7 +526,7 @@ __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
             ok = wait_phase(&ctl.kfull[i % NK], (i / NK) & 1, stop);
             if (!ok) return;
             ptx::tc_fence_after();
-            issue_scores<T>(q, kr + (i % NK) * (PAGE_BYTES >> 4), tmem + 64 * (i % SB));
+            issue_scores<C>(q, kr + (i % NK) * (C::SLOT >> 4), tmem + 64 * (i % SB));
             ptx::tc_commit(&ctl.kempty[i % NK]);
             ptx::tc_commit(&ctl.sfull[i & 1]);
         };
@@ -428,7 +543,7 @@ __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
                 if (i == 0 && seg > 0) ok = ok && wait_phase(&ctl.ofree, (seg - 1) & 1, stop);
                 if (!ok) break;
                 ptx::tc_fence_after();
-                issue_pv<T>(tmem + 64 * (it % SB), vr + (it % NV) * (PAGE_BYTES >> 4), tmem + COL_O, i == 0);
+                issue_pv<C>(tmem + 64 * (it % SB), vr + (it % NV) * (C::SLOT >> 4), tmem + COL_O, i == 0);
                 ptx::tc_commit(&ctl.vempty[it % NV]);
                 ptx::tc_commit(&ctl.odone[it & 1]);
             }
@@ -442,6 +557,7 @@ __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
         const float inv_group = 1.f / a.group;
         const int r = SPLIT > 1 ? lane : tid;  // row of the tile
         uint32_t it = 0;
+        int seg = 0;
         bool ok = true;
         do {
             const int live = min(ROWS, w.q.n * a.group - row0);
@@ -450,7 +566,7 @@ __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
             const bool active = SPLIT > 1 ? warp < SPLIT : warp * 32 < live, mine = active && r < live;
             const int node = div_small(g, inv_group), head = w.h * a.group + g - node * a.group;
             if (!a.q_tma) {
-                load_q(a, w, row0, live, inv_group, sm, tid, (const T*)nullptr);
+                load_q<C, T>(a, w, row0, live, inv_group, sm, tid);
                 ptx::fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(&ctl.qfull);
@@ -467,7 +583,7 @@ __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
                 const bool there = (unsigned)page < (unsigned)a.pages;
                 const bool edge = !there || (p + 1) * PAGE > w.q.ctx;
                 if (i + 1 < n) page = pt[p + 1];
-                if (edge && ok) {
+                if (!C::POOL_F32 && edge && ok) {
                     ok = wait_phase(&ctl.vfull[it % NV], (it / NV) & 1, stop);
                     if (ok) {
                         odd |= clean_v(vring + (it % NV) * PAGE_BYTES, max(0, w.q.ctx - p * PAGE),
@@ -587,9 +703,11 @@ __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
             ok = all_of<128>(ok);
             if (!ok) break;
             ptx::tc_fence_after();
+            if (C::POOL_F32) odd = *(volatile int*)&ctl.odd[seg & 3] == seg + 1;
+            ++seg;
             odd = !all_of<128>(!odd);
             if (active) {
-                if (odd && (SPLIT == 1 || warp == 0)) add_odd<T>(a, w, g, mine, m == -INFINITY ? 0.f : m, t_lane + COL_O);
+                if (odd && (SPLIT == 1 || warp == 0)) add_odd<T, KV>(a, w, g, mine, m == -INFINITY ? 0.f : m, t_lane + COL_O);
                 const bool whole = w.whole();
                 const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);  // 0: nothing seen
                 const size_t part = (((size_t)worker * a.lanes + tile) * 2 + w.slot()) * ROWS + r;
@@ -646,29 +764,40 @@ __global__ void __launch_bounds__(T_THREADS, TC_CTAS_PER_SM)
     if (warp == W_MMA) ptx::tmem_dealloc(tmem, TMEM_COLS);
 }
 
-template <typename T>
+template <typename T, typename KV>
 jl_status launch(const Args& a, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& q, cudaStream_t st) {
-    return launch_pdl(k_tree_attn_tc<T>, dim3(a.workers, a.lanes), dim3(T_THREADS), tc_smem<T>(), st, a, k, v, q);
+    using C = Cfg<T, KV>;
+    return launch_pdl(k_tree_attn_tc<T, KV>, dim3(a.workers, a.lanes), dim3(C::THREADS), tc_smem<C>(), st, a, k, v, q);
+}
+
+template <typename T, typename KV>
+jl_status configure() {
+    JL_CUDA(cudaFuncSetAttribute(k_tree_attn_tc<T, KV>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tc_smem<Cfg<T, KV>>()));
+    return JL_OK;
 }
 
 }  // namespace
 
 jl_status tc_configure() {
-    JL_CUDA(cudaFuncSetAttribute(k_tree_attn_tc<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tc_smem<float>()));
-    JL_CUDA(cudaFuncSetAttribute(k_tree_attn_tc<uint16_t>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 (int)tc_smem<uint16_t>()));
-    return JL_OK;
+    JL_TRY((configure<float, uint16_t>()));
+    JL_TRY((configure<uint16_t, uint16_t>()));
+    JL_TRY((configure<float, float>()));
+    return configure<uint16_t, float>();
 }
 
-jl_status tc_launch(Args a, bool f32, cudaStream_t st) {
+jl_status tc_launch(Args a, bool rows_f32, bool pool_f32, cudaStream_t st) {
+    CUtensorMap k{}, v{}, q{};
+    a.q_tma = 0;
+    if (pool_f32) return rows_f32 ? launch<float, float>(a, k, v, q, st) : launch<uint16_t, float>(a, k, v, q, st);
     const uint64_t rows = (uint64_t)a.pages * a.kv_heads * PAGE;
-    CUtensorMap k, v, q{};
-    JL_TRY(kv_page_map(&k, const_cast<void*>(a.k), rows));
-    JL_TRY(kv_page_map(&v, const_cast<void*>(a.v), rows));
+    JL_TRY(kv_page_map(&k, a.k, rows));
+    JL_TRY(kv_page_map(&v, a.v, rows));
+    if (rows_f32) return launch<float, uint16_t>(a, k, v, q, st);
     // bf16 queries by TMA: rows (node, head of the group) of a tile are one box
-    a.q_tma = !f32 && tc_tile_rows(false) % a.group == 0;
-    if (a.q_tma) JL_TRY(q_row_map(&q, a.q, a.q_heads, a.rows, a.q_ld, a.group, tc_tile_rows(false) / a.group));
-    return f32 ? launch<float>(a, k, v, q, st) : launch<uint16_t>(a, k, v, q, st);
+    const int tile = tc_tile_rows(false, false);
+    a.q_tma = tile % a.group == 0;
+    if (a.q_tma) JL_TRY(q_row_map(&q, a.q, a.q_heads, a.rows, a.q_ld, a.group, tile / a.group));
+    return launch<uint16_t, uint16_t>(a, k, v, q, st);
 }
 
 }  // namespace tree
