@@ -522,8 +522,12 @@ __global__ void __launch_bounds__(Cfg<T, KV>::THREADS, Cfg<T, KV>::CTAS)
         const uint32_t vr = desc_lo(ptx::smem_u32(vring), BOX_BYTES);
         uint32_t it = 0, seg = 0;
         bool ok = true;
+        // A wait costs a few hundred cycles even when it is over: those that are
+        // over early are made while the weights are still being computed.
+        bool k_here = false;  // the next page's K was seen
         auto scores = [&](uint32_t i) {
-            ok = wait_phase(&ctl.kfull[i % NK], (i / NK) & 1, stop);
+            if (!k_here) ok = wait_phase(&ctl.kfull[i % NK], (i / NK) & 1, stop);
+            k_here = false;
             if (!ok) return;
             ptx::tc_fence_after();
             issue_scores<C>(q, kr + (i % NK) * (C::SLOT >> 4), tmem + 64 * (i % SB));
@@ -537,10 +541,11 @@ __global__ void __launch_bounds__(Cfg<T, KV>::THREADS, Cfg<T, KV>::CTAS)
             if (ok) scores(it);
             for (int i = 0; ok && i < n; ++i, ++it) {
                 if (i + 1 < n) scores(it + 1);
-                ok = ok && wait_phase(&ctl.pfull[it & 1], (it >> 1) & 1, stop) &&
-                     wait_phase(&ctl.vfull[it % NV], (it / NV) & 1, stop);
+                ok = ok && wait_phase(&ctl.vfull[it % NV], (it / NV) & 1, stop);
                 // the last segment's O was read
                 if (i == 0 && seg > 0) ok = ok && wait_phase(&ctl.ofree, (seg - 1) & 1, stop);
+                if (i + 2 < n) k_here = ptx::mbar_try_wait(&ctl.kfull[(it + 2) % NK], ((it + 2) / NK) & 1);
+                ok = ok && wait_phase(&ctl.pfull[it & 1], (it >> 1) & 1, stop);
                 if (!ok) break;
                 ptx::tc_fence_after();
                 issue_pv<C>(tmem + 64 * (it % SB), vr + (it % NV) * (C::SLOT >> 4), tmem + COL_O, i == 0);
