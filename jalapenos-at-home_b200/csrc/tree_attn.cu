@@ -52,19 +52,24 @@ __global__ void __launch_bounds__(CB_T, CB_PER_SM) k_tree_combine(Args a) {
     __shared__ float4 share_o[CB_WARPS][32];
     __shared__ float2 share_ml[CB_WARPS];
     __shared__ int before[CB_MOST + 1];  // groups of CB_WARPS rows before item i
-    __shared__ short who[CB_MOST];       // item i is ws_join[who[i]]
+    __shared__ short who[CB_MOST];       // item i is ws_join[who[i]], kept in joins[i]
+    __shared__ int4 joins[CB_MOST];
     __shared__ int2 warp_sums[CB_WARPS];
     const int t = threadIdx.x, warp = t >> 5, l = t & 31;
     ptx::grid_dependency_wait();
     ptx::launch_dependents();
     // items and their groups of rows: thread t's workers are CB_EACH t ..
     int some = 0, groups = 0, mine[CB_EACH];
+    int4 join[CB_EACH];
 #pragma unroll
     for (int e = 0; e < CB_EACH; ++e) {
         const int w = t * CB_EACH + e;
-        const int4 join = w > 0 && w < a.workers ? a.ws_join[w] : make_int4(0, 0, 0, 0);
-        const int rows = join.w > 0 ? join.y * a.group : 0;
-        mine[e] = join.w >= CB_SHARE ? rows : (rows + CB_ROWS - 1) / CB_ROWS;
+        join[e] = w > 0 && w < a.workers ? a.ws_join[w] : make_int4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int e = 0; e < CB_EACH; ++e) {
+        const int rows = join[e].w > 0 ? join[e].y * a.group : 0;
+        mine[e] = join[e].w >= CB_SHARE ? rows : (rows + CB_ROWS - 1) / CB_ROWS;
     }
 #pragma unroll
     for (int e = 0; e < CB_EACH; ++e) {
@@ -91,6 +96,7 @@ __global__ void __launch_bounds__(CB_T, CB_PER_SM) k_tree_combine(Args a) {
     for (int e = 0; e < CB_EACH; ++e)
         if (mine[e] > 0) {
             who[item] = (short)(t * CB_EACH + e);
+            joins[item] = join[e];
             before[item++] = sum;
             sum += mine[e];
         }
@@ -102,7 +108,7 @@ __global__ void __launch_bounds__(CB_T, CB_PER_SM) k_tree_combine(Args a) {
     for (int i = blockIdx.x; i < groups; i += gridDim.x) {
         while (before[item + 1] <= i) ++item;
         const int w = who[item];
-        const int4 join = a.ws_join[w];
+        const int4 join = joins[item];
         const int rows = join.y * a.group, parts = join.w, at = i - before[item];
         // partial x of query row g: worker w - 1's slot 1, then slot 0 of the workers from w on
         auto slot = [&](int x, int g) {
