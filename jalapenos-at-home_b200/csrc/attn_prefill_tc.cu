@@ -434,18 +434,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-    static bool looked = false;
-    if (!looked) {
-        looked = true;
+    // looked up once, by whichever thread comes first
+    static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
         void* p = nullptr;
         cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) ==
-                cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = (PFN_cuTensorMapEncodeTiled_v12000)p;
+        const bool found = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) ==
+                               cudaSuccess &&
+                           q == cudaDriverEntryPointSuccess;
         cudaGetLastError();
-    }
+        return found ? (PFN_cuTensorMapEncodeTiled_v12000)p : nullptr;
+    }();
     return fn;
 }
 

@@ -27,6 +27,7 @@ const char* last_error() { return g_error; }
 jl_status cuda_fail(cudaError_t e, const char* what, const char* file, int line) {
     set_error("CUDA error %s (%s) in %s at %s:%d", cudaGetErrorName(e), cudaGetErrorString(e), what,
               file, line);
+    cudaGetLastError();  // reported here: a later call must not find it
     if (e == cudaErrorMemoryAllocation) return JL_ERR_OOM;
     if (e == cudaErrorNoDevice || e == cudaErrorInsufficientDriver) return JL_ERR_NO_DEVICE;
     return JL_ERR_CUDA;

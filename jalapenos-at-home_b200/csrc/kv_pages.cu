@@ -188,10 +188,12 @@ jl_status kv_compact(const jl_kv_compaction& a, cudaStream_t st) {
     JL_TRY(check_pages(a.pool, false));
     JL_REFUSE(a.seqs < 0 || a.seqs > 65535, "compaction: 0..65535 sequences");
     JL_REFUSE(a.path_ld < 1 || a.path_ld > JL_TREE_MAX_NODES, "compaction: path_ld must be 1..%d", JL_TREE_MAX_NODES);
+    if (a.seqs == 0) return JL_OK;
     JL_REFUSE(!a.ctx || !a.path || !a.path_len || !a.page_table,
               "compaction: ctx, path, path_len and page_table must be non-null");
     JL_REFUSE(a.max_pages < 1 || a.max_pages > MAX_TABLE, "compaction: max_pages must be 1..%d", MAX_TABLE);
-    if (a.seqs == 0) return JL_OK;
+    JL_REFUSE(words_misaligned(a.ctx, a.path, a.path_len, a.page_table, a.status),
+              "compaction: ctx, path, path_len, page_table and status must be 4-byte aligned");
     DeviceOf on;
     JL_TRY(on.enter(a.pool.k, "compaction: pool.k"));
     const int row_bytes = HEAD * (a.pool.dtype == JL_KV_F32 ? 4 : 2);

@@ -20,7 +20,12 @@ namespace jl {
 
 constexpr int MAX_TABLE = 1 << 24;  // pages of one sequence: positions fit 32 bits
 
-inline bool misaligned(const void* p) { return ((uintptr_t)p & 15) != 0; }
+inline bool misaligned(const void* p, uintptr_t to = 16) { return ((uintptr_t)p & (to - 1)) != 0; }
+// Whether any of the arrays of 32-bit numbers is not aligned as such.
+template <typename... P>
+bool words_misaligned(P... p) {
+    return (misaligned(p, 4) || ...);
+}
 
 // A pool's description; `one` for calls that work on one layer.
 jl_status check_pages(const jl_kv_pages& p, bool one);

@@ -241,6 +241,7 @@ jl_status check_sizes(const jl_tree_attn& a) {
 
 jl_status tree_attention(const jl_tree_attn& a, cudaStream_t st) {
     JL_TRY(check_sizes(a));
+    if (a.rows == 0 || a.seqs == 0) return JL_OK;
     JL_REFUSE(!a.q || !a.out || !a.row_start || !a.ctx || !a.page_table,
               "tree attention: q, out, row_start, ctx and page_table must be non-null");
     const size_t width = (size_t)a.q_heads * HEAD;
@@ -254,7 +255,8 @@ jl_status tree_attention(const jl_tree_attn& a, cudaStream_t st) {
     JL_REFUSE((long long)a.seqs * a.pool.kv_heads * (a.max_pages + SEG) >= (1ll << 31),
               "tree attention: seqs * kv heads * max_pages must stay below 2^31");
     JL_REFUSE(!(a.scale >= 0.f) || std::isinf(a.scale), "tree attention: scale must be finite and not negative");
-    if (a.rows == 0 || a.seqs == 0) return JL_OK;
+    JL_REFUSE(misaligned(a.mask, 8) || words_misaligned(a.lse, a.row_start, a.ctx, a.page_table, a.status),
+              "tree attention: mask must be 8-byte aligned, lse, row_start, ctx, page_table and status 4-byte aligned");
     DeviceOf on;
     JL_TRY(on.enter(a.pool.k, "tree attention: pool.k"));
     JL_TRY(configure(on.device));

@@ -176,6 +176,7 @@ jl_status qk_norm_rope(const jl_norm_rope& a, cudaStream_t st) {
     JL_TRY(check_pages(a.pool, true));
     JL_REFUSE(a.q_heads < 1, "norm and rotation: at least one query head");
     JL_REFUSE(a.dtype != JL_KV_BF16 && a.dtype != JL_KV_F32, "norm and rotation: dtype must be bf16 or f32");
+    if (a.rows == 0) return JL_OK;
     JL_REFUSE(!a.qkv || !a.q || !a.rope || !a.pos || !a.page_table,
               "norm and rotation: qkv, q, rope, pos and page_table must be non-null");
     const size_t in = ((size_t)a.q_heads + 2 * (size_t)a.pool.kv_heads) * HEAD, out = (size_t)a.q_heads * HEAD;
@@ -190,7 +191,8 @@ jl_status qk_norm_rope(const jl_norm_rope& a, cudaStream_t st) {
               "norm and rotation: at least one sequence and 1..%d pages each", MAX_TABLE);
     JL_REFUSE(a.positions < 1, "norm and rotation: at least one position in the rotation table");
     JL_REFUSE(!(a.eps >= 0.f), "norm and rotation: eps must not be negative");
-    if (a.rows == 0) return JL_OK;
+    JL_REFUSE(words_misaligned(a.pos, a.slot, a.seq, a.page_table, a.status),
+              "norm and rotation: pos, slot, seq, page_table and status must be 4-byte aligned");
     DeviceOf on;
     JL_TRY(on.enter(a.pool.k, "norm and rotation: pool.k"));
     RowArgs k{a.qkv,  a.q,        (long long)a.qkv_ld, (long long)a.q_ld, a.rows, a.q_heads, a.pool.kv_heads, a.seqs, a.max_pages,

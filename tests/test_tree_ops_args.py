@@ -64,7 +64,9 @@ def test_pools(call, kw, words):
     (dict(max_nodes=257), "max_nodes"), (dict(dtype=2), "dtype"), (dict(mask=P, mask_words=0), "mask"),
     (dict(mask=P, mask_words=1, max_nodes=65), "mask"), (dict(max_pages=0), "max_pages"),
     (dict(max_pages=(1 << 24) + 1), "max_pages"), (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"),
-    (dict(scale=float("inf")), "scale"), (dict(out=P, out_ld=520), "out over q")])
+    (dict(scale=float("inf")), "scale"), (dict(out=P, out_ld=520), "out over q"), (dict(mask=P + 4, mask_words=1), "8-byte"),
+    (dict(ctx=P + 2), "4-byte"), (dict(row_start=P + 1), "4-byte"), (dict(page_table=P + 2), "4-byte"), (dict(lse=P + 2), "4-byte"),
+    (dict(status=P + 2), "4-byte"), (dict(seqs=1 << 20, max_pages=1 << 20), "2^31")])
 def test_tree_attention(kw, words):
     refused(attn, words=words, **kw)
 
@@ -75,7 +77,8 @@ def test_tree_attention(kw, words):
     (dict(qkv_ld=1023), "qkv_ld"), (dict(qkv_ld=1000), "qkv_ld"), (dict(q_ld=500), "q_ld"), (dict(rows=-1), "negative"),
     (dict(q_heads=0), "query head"), (dict(dtype=5), "dtype"), (dict(seqs=0), "sequence"), (dict(max_pages=0), "pages"),
     (dict(positions=0), "position"), (dict(eps=-1e-6), "eps"), (dict(eps=float("nan")), "eps"),
-    (dict(q=P, q_ld=512), "q over qkv")])
+    (dict(q=P, q_ld=512), "q over qkv"), (dict(pos=P + 2), "4-byte"), (dict(slot=P + 1), "4-byte"), (dict(seq=P + 2), "4-byte"),
+    (dict(status=P + 3), "4-byte")])
 def test_norm_rope(kw, words):
     refused(norm, words=words, **kw)
 
@@ -83,7 +86,7 @@ def test_norm_rope(kw, words):
 @pytest.mark.parametrize("kw,words", [
     (dict(ctx=0), "non-null"), (dict(path=0), "non-null"), (dict(path_len=0), "non-null"), (dict(page_table=0), "non-null"),
     (dict(seqs=-1), "sequences"), (dict(seqs=65536), "sequences"), (dict(path_ld=0), "path_ld"), (dict(path_ld=257), "path_ld"),
-    (dict(max_pages=0), "max_pages")])
+    (dict(max_pages=0), "max_pages"), (dict(path=P + 2), "4-byte"), (dict(ctx=P + 2), "4-byte")])
 def test_compaction(kw, words):
     refused(compact, words=words, **kw)
 
@@ -121,6 +124,10 @@ def test_nothing_to_do_is_not_an_error():
     attn(seqs=0)
     norm(rows=0)
     compact(seqs=0)
+    # an empty tensor has no address
+    attn(rows=0, q=0, out=0, row_start=0, ctx=0, page_table=0, workspace=0, workspace_bytes=0)
+    norm(rows=0, qkv=0, q=0, pos=0, page_table=0)
+    compact(seqs=0, ctx=0, path=0, path_len=0, page_table=0)
     J.kv_copy_pages(pool(), [], [])
 
 
