@@ -194,7 +194,7 @@ Plan plan_of(const jl_tree_attn& a, int sms) {
     Plan p;
     const int rows = a.max_nodes * (a.q_heads / a.pool.kv_heads);
     const bool rows_f32 = a.dtype == JL_KV_F32, pool_f32 = a.pool.dtype == JL_KV_F32;
-    p.tile_rows = tc_tile_rows(rows_f32, pool_f32);
+    p.tile_rows = tc_tile_rows(rows_f32);
     p.lanes = (rows + p.tile_rows - 1) / p.tile_rows;
     p.workers = std::min(CB_MOST, std::max(1, tc_ctas(pool_f32) * sms / p.lanes));
     // Whole items or split ones: whole, a worker's longest item sets the time (in

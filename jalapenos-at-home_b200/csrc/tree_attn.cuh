@@ -241,15 +241,15 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// i / d for 0 <= i < 2^15, 1 <= d <= 128, inv = 1 / d in f32: (i + 0.5) / d is at
-// least 0.5 / 128 away from a whole number, the rounding below 2^-8.
+// i / d for 0 <= i < 256 d, 1 <= d <= 128, inv = 1 / d in f32: (i + 0.5) / d is at
+// least 0.5 / 128 away from a whole number, the rounding at most 256 * 2^-23.
 __device__ __forceinline__ int div_small(int i, float inv) { return (int)(((float)i + 0.5f) * inv); }
 
 constexpr float LN2 = 0.6931471805599453f;
 
 // The attention kernel (tree_attn_tc.cu): query rows of a tile, CTAs per SM, and
 // the launch, by the types of the rows (q and out) and of the pool.
-constexpr int tc_tile_rows(bool rows_f32, bool pool_f32) { return rows_f32 || pool_f32 ? 32 : 128; }
+constexpr int tc_tile_rows(bool rows_f32) { return rows_f32 ? 32 : 128; }
 constexpr int tc_ctas(bool pool_f32) { return pool_f32 ? 1 : 2; }
 jl_status tc_configure();
 jl_status tc_launch(Args a, bool rows_f32, bool pool_f32, cudaStream_t st);

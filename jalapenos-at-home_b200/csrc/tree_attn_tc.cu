@@ -17,9 +17,9 @@
 // row r's three bf16 pieces (24 bits), so that one MMA of 128 rows multiplies
 // all pieces.  Warps 0-2 exchange their parts of S through shared memory, all
 // compute the same weights, and warp p writes the weights' piece p; the three
-// parts of O are added at the end.  Against three MMAs a product with all pieces
-// in the rows of one tile of 64, a page takes a third of the MMA time (16
-// sequences of 8 nodes and 4 heads a KV head at 2000 positions: MEASURED).
+// parts of O are added at the end.  (Three MMAs a product, with every piece in
+// the columns of 64 rows, took 86 us for 16 sequences of 8 nodes and 4 heads a KV
+// head at 2000 positions; stacked 66.)
 // Sums, maxima and O are f32.  V rows past the sequence, and values of tree
 // nodes that are not finite, are cleared in shared memory before P V (zero
 // times them would be NaN in rows that do not see them); rows that do see such
@@ -28,10 +28,25 @@
 // which arrive as zeros, and masked.
 //
 // Pools of f32 pages: eight warps take the place of the TMA warp.  They load a
-// head's K or V rows into registers, two pages' worth ahead, and write them to
-// the rings as three bf16 pieces by truncation (24 bits, exact), so S and O take
-// three MMA groups a page; the rows are stacked as above whatever their type,
-// and one CTA fills an SM.  Clearing V happens on the way.
+// head's K or V rows into registers, two items ahead, and write them to the rings
+// as bf16 pieces, which S and O then sum: three (24 bits, exact), but two of V for
+// bf16 rows (2^-16 of a value at most, far below the output's rounding).  One CTA
+// fills an SM.  Clearing V happens on the way.
+//
+// B200, times with the joining kernel, pools of bf16: 32 sequences of 64 nodes,
+// 32 heads over 8, at 4096 positions 227 us (610 TFLOP/s of the attention's own
+// products, 914 with the second piece); one of 16 nodes at 40000 positions 44 us,
+// 37 of one node at 4096 positions 110 us (5.6 TB/s, 86% of the copy rate).
+// Small trees over long contexts are bound by the pages' bytes (1.45 us a page
+// and CTA is the copy rate), large ones by the MMAs, whose issuing thread is held
+// up by the pipe two thirds of the time; short ones by the chain of lookups,
+// copies and first instructions (about 6 us) and by the joining kernel (5 us).
+// Tried and not kept: eight softmax warps, two threads a row (272 -> 297 us for
+// the first case: exchanging the maxima costs more than it saves); the scores of
+// two pages as one MMA group of 128 columns (227 -> 252 us: the next scores no
+// longer overlap the softmax); output rows written as whole lines by way of
+// shared memory (44 -> 48 us for the second); half of the exponentials left out
+// changed nothing.
 #include <cuda.h>
 #include <cuda_bf16.h>
 
@@ -55,19 +70,18 @@ constexpr uint32_t WAIT_POLLS = 1u << 20;
 constexpr float MOVE = 8.f;  // log2 of how far a row's maximum may grow before it is moved
 
 // T: type of the rows, KV: of the pool.  SPLIT: warps that hold the pieces of the
-// same rows.  NP: pieces of the weights in a row's columns.  KVP: pieces of a
-// page.  LOADERS: warps that bring the pages.
+// same rows.  NP: pieces of the weights in a row's columns.  KP, VP: pieces
+// of a page.  LOADERS: warps that bring the pages.
 template <typename T, typename KV>
 struct Cfg {
     static constexpr bool ROWS_F32 = sizeof(T) == 4, POOL_F32 = sizeof(KV) == 4;
-    static constexpr int SPLIT = ROWS_F32 || POOL_F32 ? 3 : 1, NP = SPLIT > 1 ? 1 : 2, KVP = POOL_F32 ? 3 : 1;
-    static constexpr int ROWS = tc_tile_rows(ROWS_F32, POOL_F32), Q_ROWS = SPLIT > 1 ? SPLIT * ROWS : 128;
-    static constexpr int NK = SPLIT > 1 ? 2 : 3, NV = POOL_F32 ? 1 : 2;
+    static constexpr int SPLIT = ROWS_F32 ? 3 : 1, NP = SPLIT > 1 ? 1 : 2, KP = POOL_F32 ? 3 : 1, VP = !POOL_F32 ? 1 : ROWS_F32 ? 3 : 2;
+    static constexpr int ROWS = tc_tile_rows(ROWS_F32), Q_ROWS = SPLIT > 1 ? SPLIT * ROWS : 128;
+    static constexpr int NK = SPLIT > 1 || POOL_F32 ? 2 : 3, NV = POOL_F32 && ROWS_F32 ? 1 : 2;
     static constexpr int XCH = SPLIT > 1 ? SPLIT * ROWS * 64 * 4 : 0;  // the exchange: 64 floats of every row and part
     static constexpr int LOADERS = POOL_F32 ? 8 : 1, THREADS = 32 * (5 + LOADERS), CTAS = tc_ctas(POOL_F32);
-    static constexpr uint32_t SLOT = KVP * PAGE_BYTES;
+    static constexpr uint32_t KSLOT = KP * PAGE_BYTES, VSLOT = VP * PAGE_BYTES;
 };
-static_assert(Cfg<float, float>::ROWS == 32 && Cfg<uint16_t, uint16_t>::ROWS == 128, "tiles");
 constexpr int SB = 2;  // S buffers
 
 template <typename C>
@@ -86,10 +100,10 @@ struct Ctl {
 template <typename C>
 constexpr uint32_t q_bytes() { return C::Q_ROWS * HEAD * 2; }
 template <typename C>
-constexpr size_t tc_smem() { return q_bytes<C>() + (size_t)(C::NK + C::NV) * C::SLOT + C::XCH + 1024; }
+constexpr size_t tc_smem() { return q_bytes<C>() + (size_t)C::NK * C::KSLOT + (size_t)C::NV * C::VSLOT + C::XCH + 1024; }
 static_assert(sizeof(Ctl<Cfg<uint16_t, uint16_t>>) <= 1024, "control block");
 static_assert(tc_smem<Cfg<float, uint16_t>>() <= 113 * 1024 && tc_smem<Cfg<uint16_t, uint16_t>>() <= 113 * 1024, "two CTAs an SM");
-static_assert(tc_smem<Cfg<float, float>>() <= 227 * 1024, "one CTA an SM");
+static_assert(tc_smem<Cfg<float, float>>() <= 227 * 1024 && tc_smem<Cfg<uint16_t, float>>() <= 227 * 1024, "one CTA an SM");
 
 // Waits for a phase, for WAIT_POLLS polls or until another role stops.
 __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volatile int* stop) {
@@ -149,13 +163,7 @@ __device__ __forceinline__ void load_q(const Args& a, const Walk& w, int row0, i
         for (int i = tid; i < C::ROWS * 32; i += 128) {
             const int r = i >> 5, c = i & 31;
             if (r >= live) break;
-            float4 v;
-            if constexpr (sizeof(T) == 4) {
-                v = *(const float4*)(row(r) + 4 * c);
-            } else {
-                const uint2 u = *(const uint2*)(row(r) + 4 * c);
-                v = make_float4(lo_f(u.x), hi_f(u.x), lo_f(u.y), hi_f(u.y));
-            }
+            float4 v = *(const float4*)(row(r) + 4 * c);
 #pragma unroll
             for (int p = 0; p < C::SPLIT; ++p) {  // lanes ROWS p + r
                 const uint32_t x = pack_bf16(v.x, v.y), y = pack_bf16(v.z, v.w);
@@ -179,13 +187,13 @@ template <typename C>
 __device__ __forceinline__ void issue_scores(uint32_t q, uint32_t k, uint32_t tmem_s) {
     const uint32_t idesc = ptx::bf16_idesc(128, PAGE);
 #pragma unroll
-    for (int p = C::KVP - 1; p >= 0; --p)
+    for (int p = C::KP - 1; p >= 0; --p)
 #pragma unroll
         for (int db = 0; db < 2; ++db)
 #pragma unroll
             for (int s = 0; s < 4; ++s)
                 ptx::mma_bf16(tmem_s, desc(q + ((db * C::Q_ROWS * 128 + 32 * s) >> 4)),
-                              desc(k + ((p * PAGE_BYTES + db * BOX_BYTES + 32 * s) >> 4)), idesc, (p < C::KVP - 1 || db || s) ? 1u : 0u);
+                              desc(k + ((p * PAGE_BYTES + db * BOX_BYTES + 32 * s) >> 4)), idesc, (p < C::KP - 1 || db || s) ? 1u : 0u);
 }
 
 // The exchange between the warps that hold the pieces of 32 f32 rows: floats
@@ -205,13 +213,16 @@ template <typename C>
 __device__ __forceinline__ void issue_pv(uint32_t tmem_p, uint32_t v, uint32_t tmem_o, bool first) {
     const uint32_t idesc = ptx::bf16_idesc(128, HEAD) | (1u << 16);
 #pragma unroll
-    for (int vp = C::KVP - 1; vp >= 0; --vp)
+    for (int vp = C::VP - 1; vp >= 0; --vp)
 #pragma unroll
-        for (int p = C::NP - 1; p >= 0; --p)
+        for (int p = C::NP - 1; p >= 0; --p) {
+            if (vp && p) continue;  // both second pieces: below what two pieces leave
 #pragma unroll
-            for (int s = 0; s < 4; ++s)  // keys 16 s ..
-                ptx::mma_bf16_ta(tmem_o, tmem_p + 32 * p + 8 * s, desc(v + ((vp * PAGE_BYTES + 2048 * s) >> 4)), idesc,
-                                 (vp < C::KVP - 1 || p < C::NP - 1 || s || !first) ? 1u : 0u);
+            for (int s = 0; s < 4; ++s) {  // keys 16 s ..
+                ptx::mma_bf16_ta(tmem_o, tmem_p + 32 * p + 8 * s, desc(v + ((vp * PAGE_BYTES + 2048 * s) >> 4)), idesc, first ? 0u : 1u);
+                first = false;
+            }
+        }
 }
 
 __device__ __forceinline__ bool odd_bf16(uint32_t h) { return (h & 0x7f80u) == 0x7f80u; }  // infinite or NaN
@@ -335,10 +346,14 @@ struct Items {
     }
 };
 
-// One float4 of a row as three pieces by truncation, each the next 8 bits.
-__device__ __forceinline__ void store_pieces(uint8_t* dst, float4 x) {
+// One float4 of a row as n <= N pieces by truncation, each the next 8 bits.  (The
+// last piece rounded: 552 -> 716 us for 4 sequences of 60 nodes, 64 f32 heads over
+// 8, at 2000 positions; the conversions hold the loaders up.)
+template <int N>
+__device__ __forceinline__ void store_pieces(uint8_t* dst, float4 x, int n) {
 #pragma unroll
-    for (int p = 0; p < 3; ++p) {
+    for (int p = 0; p < N; ++p) {
+        if (p >= n) break;
         const uint32_t u0 = __float_as_uint(x.x), u1 = __float_as_uint(x.y), u2 = __float_as_uint(x.z), u3 = __float_as_uint(x.w);
         *(uint2*)(dst + p * PAGE_BYTES) = make_uint2(__byte_perm(u0, u1, 0x7632), __byte_perm(u2, u3, 0x7632));
         x = make_float4(x.x - hi_f(u0), x.y - hi_f(u1), x.z - hi_f(u2), x.w - hi_f(u3));
@@ -384,8 +399,8 @@ __global__ void __launch_bounds__(Cfg<T, KV>::THREADS, Cfg<T, KV>::CTAS)
     constexpr int ROWS = C::ROWS, NK = C::NK, NV = C::NV, NP = C::NP, SPLIT = C::SPLIT;
     extern __shared__ __align__(1024) uint8_t sm[];
     uint8_t* kring = sm + q_bytes<C>();
-    uint8_t* vring = kring + NK * C::SLOT;
-    uint8_t* xch = vring + NV * C::SLOT;
+    uint8_t* vring = kring + NK * C::KSLOT;
+    uint8_t* xch = vring + NV * C::VSLOT;
     Ctl<C>& ctl = *(Ctl<C>*)(xch + C::XCH);
     volatile int* stop = &ctl.stop;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -451,7 +466,7 @@ __global__ void __launch_bounds__(Cfg<T, KV>::THREADS, Cfg<T, KV>::CTAS)
                 ok = wait_phase(i.is_v ? &ctl.vempty[slot] : &ctl.kempty[slot], (round + 1) & 1, stop);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                uint8_t* dst = (i.is_v ? vring : kring) + slot * C::SLOT + (lane >> 4) * BOX_BYTES;
+                uint8_t* dst = (i.is_v ? vring + slot * C::VSLOT : kring + slot * C::KSLOT) + (lane >> 4) * BOX_BYTES;
                 bool odd = false;
 #pragma unroll
                 for (int k = 0; k < PAGE / 8; ++k) {
@@ -461,7 +476,7 @@ __global__ void __launch_bounds__(Cfg<T, KV>::THREADS, Cfg<T, KV>::CTAS)
                         odd = true;
                         v = make_float4(isfinite(v.x) ? v.x : 0.f, isfinite(v.y) ? v.y : 0.f, isfinite(v.z) ? v.z : 0.f, isfinite(v.w) ? v.w : 0.f);
                     }
-                    store_pieces(dst + swz128((uint32_t)r, (uint32_t)(lane & 15) * 8), v);
+                    store_pieces<C::KP>(dst + swz128((uint32_t)r, (uint32_t)(lane & 15) * 8), v, i.is_v ? C::VP : C::KP);
                 }
                 if (odd) *(volatile int*)&ctl.odd[i.seg & 3] = i.seg + 1;
                 ptx::fence_proxy_async_smem();
@@ -530,7 +545,7 @@ __global__ void __launch_bounds__(Cfg<T, KV>::THREADS, Cfg<T, KV>::CTAS)
             k_here = false;
             if (!ok) return;
             ptx::tc_fence_after();
-            issue_scores<C>(q, kr + (i % NK) * (C::SLOT >> 4), tmem + 64 * (i % SB));
+            issue_scores<C>(q, kr + (i % NK) * (C::KSLOT >> 4), tmem + 64 * (i % SB));
             ptx::tc_commit(&ctl.kempty[i % NK]);
             ptx::tc_commit(&ctl.sfull[i & 1]);
         };
@@ -548,7 +563,7 @@ __global__ void __launch_bounds__(Cfg<T, KV>::THREADS, Cfg<T, KV>::CTAS)
                 ok = ok && wait_phase(&ctl.pfull[it & 1], (it >> 1) & 1, stop);
                 if (!ok) break;
                 ptx::tc_fence_after();
-                issue_pv<C>(tmem + 64 * (it % SB), vr + (it % NV) * (C::SLOT >> 4), tmem + COL_O, i == 0);
+                issue_pv<C>(tmem + 64 * (it % SB), vr + (it % NV) * (C::VSLOT >> 4), tmem + COL_O, i == 0);
                 ptx::tc_commit(&ctl.vempty[it % NV]);
                 ptx::tc_commit(&ctl.odone[it & 1]);
             }
@@ -799,7 +814,7 @@ jl_status tc_launch(Args a, bool rows_f32, bool pool_f32, cudaStream_t st) {
     JL_TRY(kv_page_map(&v, a.v, rows));
     if (rows_f32) return launch<float, uint16_t>(a, k, v, q, st);
     // bf16 queries by TMA: rows (node, head of the group) of a tile are one box
-    const int tile = tc_tile_rows(false, false);
+    const int tile = tc_tile_rows(false);
     a.q_tma = tile % a.group == 0;
     if (a.q_tma) JL_TRY(q_row_map(&q, a.q, a.q_heads, a.rows, a.q_ld, a.group, tile / a.group));
     return launch<uint16_t, uint16_t>(a, k, v, q, st);
