@@ -375,7 +375,9 @@ jl_status jl_qk_norm_rope(const jl_norm_rope* a, void* stream);
  *   once into the output type; lse = log of the sum of exp(q . k_p * scale).
  * A row that sees nothing gets zeros and an lse of -infinity.  Whatever lies
  * in positions that a row does not see, infinities and NaN included, does
- * not reach its output.  Rows from row_start[seqs] on are not written.
+ * not reach its output; a value that is not finite in a position that it sees
+ * makes that dim of its output infinite or NaN, whatever the position's
+ * weight.  Rows from row_start[seqs] on are not written.
  * The sum is split between CTAs by the lengths of the whole batch, in a
  * fixed order: the same inputs give the same bits, but a row's last bits may
  * differ in another batch. */
