@@ -15,21 +15,30 @@
 
 namespace jl {
 
+// `cluster`: CTAs of a cluster along x (1: none).
 template <typename... KArgs, typename... Args>
-jl_status launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
-                     cudaStream_t stream, Args&&... args) {
+jl_status launch_pdl_cluster(void (*kernel)(KArgs...), int cluster, dim3 grid, dim3 block, size_t smem,
+                             cudaStream_t stream, Args&&... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     JL_CUDA(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
     return JL_OK;
+}
+template <typename... KArgs, typename... Args>
+jl_status launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
+                     cudaStream_t stream, Args&&... args) {
+    return launch_pdl_cluster(kernel, 1, grid, block, smem, stream, std::forward<Args>(args)...);
 }
 
 }  // namespace jl

@@ -15,11 +15,6 @@ namespace jl {
 namespace tree {
 namespace {
 
-__device__ __forceinline__ void store4(float* p, float4 v) { *(float4*)p = v; }
-__device__ __forceinline__ void store4(uint16_t* p, float4 v) {
-    *(uint2*)p = make_uint2(f2bf16(v.x) | (uint32_t)f2bf16(v.y) << 16, f2bf16(v.z) | (uint32_t)f2bf16(v.w) << 16);
-}
-
 // ---- partial results -----------------------------------------------------------------
 //
 // The rows to add (query rows of the items that ws_join names) are dealt out
@@ -33,19 +28,6 @@ constexpr int CB_WARPS = 4, CB_T = 32 * CB_WARPS, CB_PER_SM = 5;
 constexpr int CB_MOST = 512, CB_EACH = CB_MOST / CB_T;  // workers at most; of them to a thread
 constexpr int CB_SHARE = 8;    // partials from which the warps share a row
 constexpr int CB_RPW = 2, CB_ROWS = CB_RPW * CB_WARPS;
-
-struct RowSum {
-    float top, sum;
-    float4 o;
-};
-__device__ __forceinline__ void add_part(RowSum& t, float m, float l, float4 v) {
-    if (l == 0.f) return;  // nothing seen there
-    const float top = fmaxf(t.top, m), ref = top == -INFINITY ? 0.f : top;
-    const float f = ex2(t.top - ref), g = ex2(m - ref);
-    t.top = top;
-    t.sum = fmaf(t.sum, f, l * g);
-    t.o = make_float4(fmaf(t.o.x, f, v.x * g), fmaf(t.o.y, f, v.y * g), fmaf(t.o.z, f, v.z * g), fmaf(t.o.w, f, v.w * g));
-}
 
 template <typename T>
 __global__ void __launch_bounds__(CB_T, CB_PER_SM) k_tree_combine(Args a) {
@@ -115,15 +97,7 @@ __global__ void __launch_bounds__(CB_T, CB_PER_SM) k_tree_combine(Args a) {
             const int lane = g / R;
             return ((size_t)((w - 1 + x) * a.lanes + lane) * 2 + (x == 0 ? 1 : 0)) * R + (g - lane * R);
         };
-        auto finish = [&](const RowSum& sum, int g) {
-            const float inv = sum.sum == 0.f ? 0.f : __fdiv_rn(1.f, sum.sum);
-            const int node = div_small(g, inv_group), head = join.z * a.group + g - node * a.group;
-            store4((T*)a.out + (size_t)(join.x + node) * a.out_ld + (size_t)head * HEAD + 4 * l,
-                   make_float4(sum.o.x * inv, sum.o.y * inv, sum.o.z * inv, sum.o.w * inv));
-            if (a.lse && l == 0)
-                a.lse[(size_t)(join.x + node) * a.q_heads + head] =
-                    sum.sum == 0.f ? -INFINITY : (sum.top + log2f(sum.sum)) * LN2;
-        };
+        auto finish = [&](const RowSum& sum, int g) { finish_row<T>(a, join.x, join.z, g, l, sum, inv_group); };
         if (parts < CB_SHARE) {
             float2 ml[CB_RPW][CB_SHARE - 1];
             float4 v[CB_RPW][CB_SHARE - 1];
@@ -184,45 +158,67 @@ __global__ void __launch_bounds__(CB_T, CB_PER_SM) k_tree_combine(Args a) {
 
 // ---- host ----------------------------------------------------------------------------
 
-// The kernel that a call takes and how it cuts the work.
+// What a device allows, found once.
+jl_status limits_of(int device, TcLimits& out) {
+    static std::mutex mu;
+    static TcLimits found[64];
+    static bool done[64] = {};
+    std::lock_guard<std::mutex> g(mu);
+    if (device >= 64 || !done[device]) {
+        JL_TRY(tc_configure(out));
+        if (device >= 64) return JL_OK;
+        found[device] = out;
+        done[device] = true;
+    }
+    out = found[device];
+    return JL_OK;
+}
+
+// How a call cuts the work: whole items (parts 1), items shared by clusters of
+// `parts` CTAs, or even ranges of units.
 struct Plan {
-    int tile_rows, lanes, workers, min_units, whole;
+    int tile_rows, lanes, workers, min_units, whole, parts;
     size_t bytes;
 };
 
-Plan plan_of(const jl_tree_attn& a, int sms) {
+Plan plan_of(const jl_tree_attn& a, int sms, const TcLimits& limits) {
     Plan p;
     const int rows = a.max_nodes * (a.q_heads / a.pool.kv_heads);
     const bool rows_f32 = a.dtype == JL_KV_F32, pool_f32 = a.pool.dtype == JL_KV_F32;
     p.tile_rows = tc_tile_rows(rows_f32);
     p.lanes = (rows + p.tile_rows - 1) / p.tile_rows;
     p.workers = std::min(CB_MOST, std::max(1, tc_ctas(pool_f32) * sms / p.lanes));
-    // Whole items or split ones: whole, a worker's longest item sets the time (in
-    // waves of all workers); split, the mean does, and the join is added.  The
-    // times, in us on a B200 with every SM busy, are a page's (1.5 for bf16
-    // rows and pools, 2 with f32), a segment's start and end (6) and
-    // the join (5).  Measured whole / split, 8 bf16 nodes, 32 heads over 8: one
-    // sequence of 300 positions 10.6 / 14.7 us, 32 of them 15.3 / 30.4 us, 32 of up
-    // to 700 23.6 / 34.5 us; f32 rows, one sequence of 700 29.6 / 20.9 us.
-    const double page = rows_f32 || pool_f32 ? 2.0 : 1.5;
+    p.parts = 1;
+    // Whole items or shared ones: the longest item sets the time, whose parts are
+    // added within a cluster.  Even ranges: the mean does (of a batch it is taken as
+    // 0.8 of the longest), but the join is a kernel of its own, and starts and ends
+    // of segments add up.  Times in us on a B200, fitted to calls of 32 heads over 8:
+    // of a page with one CTA an SM and with two, of a CTA's start and end, and of
+    // even ranges, which grow with the rows of a tile.  Measured, whole / 8 parts /
+    // even: one sequence of 8 bf16 nodes at 100 positions 7.5 / 9.0 / 13.0 us, at 300
+    // 11.0 / 8.6 / 14.5, at 1500 35.5 / 11.0 / 14.3, at 12000 257 / 41 / 24; four of 32
+    // nodes at 4096 97 / 30 / 44; eight of 8 nodes at 1500, four parts, 39 / 20 / 28;
+    // f32 rows and pool, four of 8 nodes at 1500, four parts, 84 / 32 / 44.
+    const double one = pool_f32 ? 3.0 : rows_f32 ? 1.4 : 1.35, two = pool_f32 ? 3.0 : rows_f32 ? 2.0 : 1.65;
+    const int r = std::min(rows, p.tile_rows);
+    const double start = (pool_f32 ? 6.0 : rows_f32 ? 7.2 : 5.2) + 0.025 * r;
     const double ctas = (double)a.seqs * a.pool.kv_heads * p.lanes, slots = (double)p.workers * p.lanes;
-    const double whole = std::ceil(ctas / slots) * (a.max_pages * page + 6);
-    const double split = std::max(ctas * (a.max_pages + SEG) / slots, 1.0 + SEG) * page + 6 + 5;
-    // sizes of 0 ask for the workspace of any call
-    p.whole = a.seqs > 0 && a.max_pages > 0 && whole <= split;
+    const double units = std::max(ctas * (a.max_pages + SEG) / slots * (a.seqs > 1 ? 0.8 : 1.0), 1.0 + SEG);
+    const double even = (pool_f32 ? 12.0 : rows_f32 ? 10.5 : 9.0) + 0.12 * r + units * (pool_f32 ? 4.4 : rows_f32 ? 2.2 : 1.9);
+    double best = std::ceil(ctas / slots) * (start + a.max_pages * (ctas > sms ? two : one));
+    p.whole = best <= even;
+    for (int i = 0, n = 2; i < TcLimits::SIZES; ++i, n *= 2) {
+        const double shared = start + 1.5 + std::ceil((double)a.max_pages / n) * (ctas * n > sms ? two : one);
+        if (ctas > limits.clusters[rows_f32][pool_f32][i] || shared >= std::min(best, even)) continue;
+        best = shared;
+        p.parts = n;
+        p.whole = 1;
+    }
+    if (a.seqs == 0 || a.max_pages == 0) p.whole = 0, p.parts = 1;  // the workspace of any call is asked for
+    if (p.parts > 1) p.workers = a.seqs * a.pool.kv_heads;
     p.min_units = p.whole ? 1 : 1 + SEG;
     p.bytes = p.workers == 1 || p.whole ? 0 : (size_t)p.workers * (sizeof(int4) + (size_t)p.lanes * 2 * p.tile_rows * (HEAD + 2) * sizeof(float));
     return p;
-}
-
-jl_status configure(int device) {  // once per device
-    static std::mutex mu;
-    static bool done[64] = {};
-    std::lock_guard<std::mutex> g(mu);
-    if (device < 64 && done[device]) return JL_OK;
-    JL_TRY(tc_configure());
-    if (device < 64) done[device] = true;
-    return JL_OK;
 }
 
 jl_status check_sizes(const jl_tree_attn& a) {
@@ -259,8 +255,9 @@ jl_status tree_attention(const jl_tree_attn& a, cudaStream_t st) {
               "tree attention: mask must be 8-byte aligned, lse, row_start, ctx, page_table and status 4-byte aligned");
     DeviceOf on;
     JL_TRY(on.enter(a.pool.k, "tree attention: pool.k"));
-    JL_TRY(configure(on.device));
-    const Plan p = plan_of(a, on.sms);
+    TcLimits limits;
+    JL_TRY(limits_of(on.device, limits));
+    const Plan p = plan_of(a, on.sms, limits);
     JL_REFUSE(p.bytes && (!a.workspace || ((uintptr_t)a.workspace & 255)),
               "tree attention: the workspace must be 256-byte aligned device memory");
     JL_REFUSE(a.workspace_bytes < p.bytes, "tree attention: workspace of %zu bytes, %zu needed", a.workspace_bytes, p.bytes);
@@ -291,6 +288,7 @@ jl_status tree_attention(const jl_tree_attn& a, cudaStream_t st) {
     k.tile_rows = p.tile_rows;
     k.min_units = p.min_units;
     k.whole = p.whole;
+    k.parts = p.parts;
     k.ws_join = (int4*)a.workspace;
     k.ws_o = (float*)(k.ws_join + p.workers);
     k.ws_ml = k.ws_o + (size_t)p.workers * p.lanes * 2 * p.tile_rows * HEAD;
@@ -311,7 +309,9 @@ jl_status tree_attention_workspace(const jl_tree_attn& a, size_t* bytes) {
     JL_TRY(check_sizes(a));
     DeviceOf on;
     JL_TRY(on.enter(a.pool.k, "tree attention: pool.k"));
-    *bytes = plan_of(a, on.sms).bytes;
+    TcLimits limits;
+    JL_TRY(limits_of(on.device, limits));
+    *bytes = plan_of(a, on.sms, limits).bytes;
     return JL_OK;
 }
 

@@ -13,8 +13,12 @@
 // two partials: the item its range starts in (slot 0) and the item its range
 // ends in (slot 1).  The first worker w whose pages start inside an item says
 // in ws_join[w] what there is to add: the partial of worker w - 1 (slot 1) and
-// those of w, w + 1 .. (slot 0).  Where no sequence can have more than a few
-// pages (`whole`), an item is one unit: none is split, and nothing is joined.
+// those of w, w + 1 .. (slot 0).
+// Where no sequence can have many pages (`whole`), an item is one unit: none is
+// cut by ranges, and nothing is joined.  If there are few items, each goes to a
+// cluster of `parts` CTAs instead of one: CTA r takes the r-th part of the
+// item's pages and leaves its rows' partial results in its shared memory, and
+// every CTA adds and writes every parts-th row.
 //
 // The query rows of an item are node * group + head of the group, cut into
 // tiles of `tile_rows`; a worker is `lanes` CTAs, one per tile, that walk the
@@ -54,7 +58,8 @@ struct Args {
     float* ws_o;       // [worker][lane][slot][tile_rows][HEAD]
     float* ws_ml;      // [worker][lane][slot][tile_rows][2]: maximum (scores times c2), sum
     int workers, lanes, tile_rows, min_units;
-    int whole;         // items are not split
+    int whole;         // items are not split over workers
+    int parts;         // CTAs of a cluster that share a worker's only item; 1: none
     int q_tma;         // the tensor-core kernel's queries come by TMA
     int32_t* status;
 };
@@ -179,6 +184,12 @@ struct Walk {
         p1 = a.whole ? q.np : min(q.np, end - item - SEG);
         return p1 > p0 || next(a);
     }
+    // Keeps part `rank` of the item's pages; false: it has none.
+    __device__ bool part(int rank, int parts) {
+        p0 = q.np * rank / parts;
+        p1 = q.np * (rank + 1) / parts;
+        return p1 > p0;
+    }
     __device__ bool next(const Args& a) {
         item += item_units(a, q);
         if (item + (a.whole ? 0 : SEG) >= end) return false;  // no page of the next item
@@ -247,11 +258,44 @@ __device__ __forceinline__ int div_small(int i, float inv) { return (int)(((floa
 
 constexpr float LN2 = 0.6931471805599453f;
 
+__device__ __forceinline__ void store4(float* p, float4 v) { *(float4*)p = v; }
+__device__ __forceinline__ void store4(uint16_t* p, float4 v) {
+    *(uint2*)p = make_uint2(f2bf16(v.x) | (uint32_t)f2bf16(v.y) << 16, f2bf16(v.z) | (uint32_t)f2bf16(v.w) << 16);
+}
+
+// A row's sum over partial results, each (maximum, sum, sums of 4 dims).
+struct RowSum {
+    float top, sum;
+    float4 o;
+};
+__device__ __forceinline__ void add_part(RowSum& t, float m, float l, float4 v) {
+    if (l == 0.f) return;  // nothing seen there
+    const float top = fmaxf(t.top, m), ref = top == -INFINITY ? 0.f : top;
+    const float f = ex2(t.top - ref), g = ex2(m - ref);
+    t.top = top;
+    t.sum = fmaf(t.sum, f, l * g);
+    t.o = make_float4(fmaf(t.o.x, f, v.x * g), fmaf(t.o.y, f, v.y * g), fmaf(t.o.z, f, v.z * g), fmaf(t.o.w, f, v.w * g));
+}
+// Query row g of an item with first row lo and KV head h: writes dims 4 l .. and
+// (lane 0) the lse.
+template <typename T>
+__device__ __forceinline__ void finish_row(const Args& a, int lo, int h, int g, int l, const RowSum& sum, float inv_group) {
+    const float inv = sum.sum == 0.f ? 0.f : __fdiv_rn(1.f, sum.sum);
+    const int node = div_small(g, inv_group), head = h * a.group + g - node * a.group;
+    store4((T*)a.out + (size_t)(lo + node) * a.out_ld + (size_t)head * HEAD + 4 * l,
+           make_float4(sum.o.x * inv, sum.o.y * inv, sum.o.z * inv, sum.o.w * inv));
+    if (a.lse && l == 0) a.lse[(size_t)(lo + node) * a.q_heads + head] = sum.sum == 0.f ? -INFINITY : (sum.top + log2f(sum.sum)) * LN2;
+}
+
 // The attention kernel (tree_attn_tc.cu): query rows of a tile, CTAs per SM, and
 // the launch, by the types of the rows (q and out) and of the pool.
 constexpr int tc_tile_rows(bool rows_f32) { return rows_f32 ? 32 : 128; }
 constexpr int tc_ctas(bool pool_f32) { return pool_f32 ? 1 : 2; }
-jl_status tc_configure();
+struct TcLimits {
+    static constexpr int SIZES = 3;
+    int clusters[2][2][SIZES];  // of 2, 4, 8 CTAs that run at once, by [rows f32][pool f32]
+};
+jl_status tc_configure(TcLimits& limits);
 jl_status tc_launch(Args a, bool rows_f32, bool pool_f32, cudaStream_t st);
 
 }  // namespace tree

@@ -15,11 +15,12 @@
 //     buffers).
 // f32 rows are stacked: a tile has 32 rows, and lanes 32 p + r hold piece p of
 // row r's three bf16 pieces (24 bits), so that one MMA of 128 rows multiplies
-// all pieces.  Warps 0-2 exchange their parts of S through shared memory, all
-// compute the same weights, and warp p writes the weights' piece p; the three
-// parts of O are added at the end.  (Three MMAs a product, with every piece in
-// the columns of 64 rows, took 86 us for 16 sequences of 8 nodes and 4 heads a KV
-// head at 2000 positions; stacked 66.)
+// all pieces.  Warps 0-2 exchange their parts of S through shared memory; each
+// adds them for a window of the keys and writes the pieces of their weights;
+// then warp p takes piece p of all keys to TMEM.  The three parts of O are added
+// at the end.  16 sequences of 8 nodes and 4 heads a KV head at 2000 positions:
+// 55 us; 66 when each warp added all parts and computed all weights, 86 with
+// three MMAs a product and every piece in the columns of 64 rows.
 // Sums, maxima and O are f32.  V rows past the sequence, and values of tree
 // nodes that are not finite, are cleared in shared memory before P V (zero
 // times them would be NaN in rows that do not see them); rows that do see such
@@ -82,7 +83,8 @@ struct Cfg {
     static constexpr int LOADERS = POOL_F32 ? 8 : 1, THREADS = 32 * (5 + LOADERS), CTAS = tc_ctas(POOL_F32);
     static constexpr uint32_t KSLOT = KP * PAGE_BYTES, VSLOT = VP * PAGE_BYTES;
 };
-constexpr int SB = 2;  // S buffers
+constexpr int SB = 2;   // S buffers
+constexpr int WIN = 24;  // keys of a warp that exchanges
 
 template <typename C>
 struct Ctl {
@@ -94,6 +96,7 @@ struct Ctl {
     // The loader warps of an f32 pool took a value out of segment s: odd[s % 4] is
     // s + 1 (they are less than four segments ahead: the rings hold three pages)
     int odd[4];
+    float tops[C::SPLIT > 1 ? 96 : 1];  // of a page's windows
     LocateScratch locate;
 };
 
@@ -101,7 +104,7 @@ template <typename C>
 constexpr uint32_t q_bytes() { return C::Q_ROWS * HEAD * 2; }
 template <typename C>
 constexpr size_t tc_smem() { return q_bytes<C>() + (size_t)C::NK * C::KSLOT + (size_t)C::NV * C::VSLOT + C::XCH + 1024; }
-static_assert(sizeof(Ctl<Cfg<uint16_t, uint16_t>>) <= 1024, "control block");
+static_assert(sizeof(Ctl<Cfg<uint16_t, uint16_t>>) <= 1024 && sizeof(Ctl<Cfg<float, float>>) <= 1024, "control block");
 static_assert(tc_smem<Cfg<float, uint16_t>>() <= 113 * 1024 && tc_smem<Cfg<uint16_t, uint16_t>>() <= 113 * 1024, "two CTAs an SM");
 static_assert(tc_smem<Cfg<float, float>>() <= 227 * 1024 && tc_smem<Cfg<uint16_t, float>>() <= 227 * 1024, "one CTA an SM");
 
@@ -179,7 +182,7 @@ __device__ __forceinline__ void load_q(const Args& a, const Walk& w, int row0, i
 // the issuing thread adds constants to it: building each descriptor from its
 // address costs more than the MMA takes.
 constexpr uint32_t DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
-__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo) { return (saddr >> 4) | ((lbo >> 4) << 16); }
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo) { return ((saddr & 0x3ffff) >> 4) | ((lbo >> 4) << 16); }
 __device__ __forceinline__ uint64_t desc(uint32_t lo) { return (uint64_t)DESC_HI << 32 | lo; }
 
 // S = Q K^T of one page, its pieces smallest first; q, k: low words.
@@ -391,6 +394,43 @@ __device__ __forceinline__ void store_row32<uint16_t>(uint16_t* dst, const float
                                         pack_bf16(o[i + 4] * f, o[i + 5] * f), pack_bf16(o[i + 6] * f, o[i + 7] * f));
 }
 
+// The parts of an item that the CTAs of a cluster hold in shared memory: 128
+// floats of each row, 16-byte units swizzled so that 8 rows lie on all banks.
+__device__ __forceinline__ uint32_t part_at(int row, int unit) { return row * (HEAD * 4) + ((unit ^ (row & 31)) << 4); }
+__device__ __forceinline__ void store_part(float* part, int row, int c, const float (&o)[32]) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 4)
+        *(float4*)((uint8_t*)part + part_at(row, (c + i) >> 2)) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+}
+// Adds them, in the order of the parts: each CTA takes every parts-th row, a
+// warp a row, lane l its dims 4 l ..
+template <typename T, int THREADS>
+__device__ __forceinline__ void add_parts(const Args& a, const Walk& w, int rank, int row0, int rows, uint32_t o, uint32_t ml) {
+    constexpr int AT_ONCE = 8;
+    const int warp = threadIdx.x >> 5, l = threadIdx.x & 31;
+    const float inv_group = 1.f / a.group;
+    for (int r = rank + a.parts * warp; r < rows; r += a.parts * (THREADS / 32)) {
+        RowSum sum{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+        for (int x = 0; x < a.parts; x += AT_ONCE) {
+            float2 s[AT_ONCE];
+            float4 v[AT_ONCE];
+#pragma unroll
+            for (int e = 0; e < AT_ONCE; ++e) {
+                s[e] = make_float2(-INFINITY, 0.f);
+                v[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (x + e < a.parts) {
+                    const uint32_t at = ptx::mapa(ml + 8 * r, x + e);
+                    s[e] = make_float2(ptx::ld_shared_cluster(at), ptx::ld_shared_cluster(at + 4));
+                    v[e] = ptx::ld_shared_cluster_v4(ptx::mapa(o + part_at(r, l), x + e));
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < AT_ONCE; ++e) add_part(sum, s[e].x, s[e].y, v[e]);
+        }
+        finish_row<T>(a, w.q.lo, w.h, row0 + r, l, sum, inv_group);
+    }
+}
+
 template <typename T, typename KV>
 __global__ void __launch_bounds__(Cfg<T, KV>::THREADS, Cfg<T, KV>::CTAS)
     k_tree_attn_tc(Args a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
@@ -404,7 +444,7 @@ __global__ void __launch_bounds__(Cfg<T, KV>::THREADS, Cfg<T, KV>::CTAS)
     Ctl<C>& ctl = *(Ctl<C>*)(xch + C::XCH);
     volatile int* stop = &ctl.stop;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int worker = blockIdx.x, tile = blockIdx.y;
+    const int worker = blockIdx.x / a.parts, rank = blockIdx.x % a.parts, tile = blockIdx.y;
     if (tid == 0) {
         for (int i = 0; i < NK; ++i) {
             ptx::mbar_init(&ctl.kfull[i], C::LOADERS);
@@ -443,8 +483,14 @@ __global__ void __launch_bounds__(Cfg<T, KV>::THREADS, Cfg<T, KV>::CTAS)
     ptx::launch_dependents();
     const Split sp = locate<C::THREADS>(a, worker, ctl.locate);
     Walk w;
-    const bool work = w.start(a, ctl.locate.found, sp.at(worker), sp.at(worker + 1)) && !(ptx::smem_u32(sm) & 1023);
+    bool work = w.start(a, ctl.locate.found, sp.at(worker), sp.at(worker + 1)) && !(ptx::smem_u32(sm) & 1023);
     const int row0 = tile * ROWS;
+    // a cluster's rows to add; the part of one without pages adds nothing
+    const int shared_rows = a.parts > 1 && work ? min(ROWS, w.q.n * a.group - row0) : 0;
+    float* part_o = (float*)sm;  // over Q and the rings, once they were read
+    float2* part_ml = (float2*)(sm + ROWS * HEAD * 4);
+    if (a.parts > 1 && work && !(work = w.part(rank, a.parts)))
+        for (int i = tid; i < shared_rows; i += C::THREADS) part_ml[i] = make_float2(-INFINITY, 0.f);
     if (tid == 0 && tile == 0 && a.workers > 1 && !a.whole) a.ws_join[worker] = w.join(sp, worker, work);
 
     if (C::POOL_F32 && work && warp >= W_LOAD) {
@@ -617,98 +663,155 @@ __global__ void __launch_bounds__(Cfg<T, KV>::THREADS, Cfg<T, KV>::CTAS)
                 ptx::tc_fence_after();
                 if (active) {
                     const uint32_t t_s = t_lane + 64 * (it % SB);
-                    float x[64];
-                    if (ok) ptx::tmem_ld64_sync(t_s, x);
-                    if constexpr (SPLIT > 1) {  // the pieces' parts of S
-                        if (ok) {
-#pragma unroll
-                            for (int c = 0; c < 64; c += 4) *xch_at(xch, warp, lane, c) = make_float4(x[c], x[c + 1], x[c + 2], x[c + 3]);
+                    // moves the row's maximum to `top` where that is due, and O and l with it
+                    auto move = [&](float top) {
+                        float f = 1.f;
+                        if (m == -INFINITY) {
+                            m = top;  // nothing was seen before: O and l are zero
+                        } else if (top > m + MOVE) {
+                            f = ex2(m - top);
+                            m = top;
+                            l *= f;
                         }
-                        ok = all_of<32 * SPLIT>(ok);
+                        if (i > 0 && __any_sync(0xffffffffu, mine && f != 1.f)) {
+                            const uint32_t j = it - 1;  // every earlier P V is done
+                            ok = __all_sync(0xffffffffu, wait_phase(&ctl.odone[j & 1], (j >> 1) & 1, stop));
+                            ptx::tc_fence_after();
+#pragma unroll 1
+                            for (int c = 0; ok && c < HEAD; c += 32) {
+                                float o[32];
+                                uint32_t b[32];
+                                ptx::tmem_ld32_sync(t_lane + COL_O + c, o);
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) b[e] = __float_as_uint(o[e] * f);
+                                ptx::tmem_st32(t_lane + COL_O + c, b);
+                            }
+                        }
+                        return m == -INFINITY ? 0.f : m;
+                    };
+                    const uint64_t vis = !edge ? ~0ull : mine && there ? visible(a, w.q, node, p, m0) : 0;
+                    // pieces by truncation: each takes the next 8 bits, exactly
+                    auto piece = [](float x, float y) { return __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632); };
+                    auto rest = [](float x, float y) {
+                        return add2(make_float2(x, y), make_float2(-hi_f(__float_as_uint(x)), -hi_f(__float_as_uint(y))));
+                    };
+                    const float2 c2 = make_float2(a.c2, a.c2);
+                    if constexpr (SPLIT > 1) {
+                        // The windows have 24 keys; the last one's first 8 are the second's too.
+                        // Code and registers are kept short here: S in halves and all
+                        // of it sent took 55 us (case above), S at once 63, and only what
+                        // others need, chosen by warp, more than the old exchange.
+                        const int c0 = warp == 2 ? 40 : 24 * warp;
+                        ok = all_of<32 * SPLIT>(ok);  // and the last page's pieces were read
                         if (!ok) break;
 #pragma unroll
-                        for (int c = 0; c < 64; c += 4) {
-                            const float4 u = xch_sum(xch, lane, c);
+                        for (int h = 0; h < 64; h += 32) {
+                            float s[32];
+                            ptx::tmem_ld32_sync(t_s + h, s);
+#pragma unroll
+                            for (int c = 0; c < 32; c += 4) *xch_at(xch, warp, lane, h + c) = make_float4(s[c], s[c + 1], s[c + 2], s[c + 3]);
+                        }
+                        all_of<32 * SPLIT>(true);
+                        float x[WIN];
+#pragma unroll
+                        for (int c = 0; c < WIN; c += 4) {
+                            const float4 u = xch_sum(xch, lane, c0 + c);
                             x[c] = u.x, x[c + 1] = u.y, x[c + 2] = u.z, x[c + 3] = u.w;
                         }
-                        all_of<32 * SPLIT>(true);  // every part was read
-                    }
-                    if (edge) {
-                        const uint64_t vis = mine && there ? visible(a, w.q, node, p, m0) : 0;
-                        const uint32_t v0 = (uint32_t)vis, v1 = (uint32_t)(vis >> 32);
+                        if (edge) {
+                            const uint32_t v = (uint32_t)(vis >> c0);
 #pragma unroll
-                        for (int c = 0; c < 32; ++c) {
-                            if (!(v0 >> c & 1)) x[c] = -INFINITY;
-                            if (!(v1 >> c & 1)) x[32 + c] = -INFINITY;
+                            for (int c = 0; c < WIN; ++c)
+                                if (!(v >> c & 1)) x[c] = -INFINITY;
                         }
-                    }
-                    float t0 = max3(x[0], x[1], x[2]), t1 = max3(x[3], x[4], x[5]);
-                    float t2 = max3(x[6], x[7], x[8]), t3 = max3(x[9], x[10], x[11]);
+                        float t0 = max3(x[0], x[1], x[2]), t1 = max3(x[3], x[4], x[5]);
 #pragma unroll
-                    for (int c = 12; c < 60; c += 8) {
-                        t0 = max3(t0, x[c], x[c + 1]);
-                        t1 = max3(t1, x[c + 2], x[c + 3]);
-                        t2 = max3(t2, x[c + 4], x[c + 5]);
-                        t3 = max3(t3, x[c + 6], x[c + 7]);
-                    }
-                    t0 = max3(t0, x[60], x[61]);
-                    t1 = max3(t1, x[62], x[63]);
-                    t0 = max3(t0, t1, t2);
-                    const float top = fmaxf(t0, t3) * a.c2;
-                    float f = 1.f;
-                    if (m == -INFINITY) {
-                        m = top;  // nothing was seen before: O and l are zero
-                    } else if (top > m + MOVE) {
-                        f = ex2(m - top);
-                        m = top;
-                        l *= f;
-                    }
-                    if (i > 0 && __any_sync(0xffffffffu, mine && f != 1.f)) {
-                        const uint32_t j = it - 1;  // every earlier P V is done
-                        ok = __all_sync(0xffffffffu, wait_phase(&ctl.odone[j & 1], (j >> 1) & 1, stop));
-                        ptx::tc_fence_after();
-#pragma unroll 1
-                        for (int c = 0; ok && c < HEAD; c += 32) {
-                            float o[32];
-                            uint32_t b[32];
-                            ptx::tmem_ld32_sync(t_lane + COL_O + c, o);
+                        for (int c = 6; c < WIN - 2; c += 4) t0 = max3(t0, x[c], x[c + 1]), t1 = max3(t1, x[c + 2], x[c + 3]);
+                        ctl.tops[warp * 32 + lane] = fmaxf(max3(t0, x[WIN - 2], x[WIN - 1]), t1);
+                        all_of<32 * SPLIT>(true);  // and every part was read
+                        const float ref = move(max3(ctl.tops[lane], ctl.tops[32 + lane], ctl.tops[64 + lane]) * a.c2);
+                        const float2 nref = make_float2(-ref, -ref);
+                        float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) b[e] = __float_as_uint(o[e] * f);
-                            ptx::tmem_st32(t_lane + COL_O + c, b);
+                        for (int q = 0; q < WIN / 8; ++q) {
+                            const bool own = q > 0 || warp < 2;
+                            uint32_t b[SPLIT][4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                float2 y = fma2(make_float2(x[8 * q + 2 * e], x[8 * q + 2 * e + 1]), c2, nref);
+                                y = make_float2(ex2(y.x), ex2(y.y));
+                                if (own) sum = add2(sum, y);
+#pragma unroll
+                                for (int k = 0; k < SPLIT; ++k) {
+                                    if (k) y = rest(y.x, y.y);
+                                    b[k][e] = piece(y.x, y.y);
+                                }
+                            }
+                            const uint32_t at = lane * 128 + (((c0 / 8 + q) ^ (lane & 7)) << 4);
+#pragma unroll
+                            for (int k = 0; k < SPLIT; ++k)
+                                if (own) *(uint4*)(xch + k * 4096 + at) = make_uint4(b[k][0], b[k][1], b[k][2], b[k][3]);
                         }
-                    }
-                    const float ref = m == -INFINITY ? 0.f : m;
-                    const float2 c2 = make_float2(a.c2, a.c2), nref = make_float2(-ref, -ref);
-                    float2 s0 = make_float2(0.f, 0.f), s1 = s0;
-#pragma unroll
-                    for (int c = 0; c < 64; c += 4) {
-                        float2 y = fma2(make_float2(x[c], x[c + 1]), c2, nref);
-                        float2 z = fma2(make_float2(x[c + 2], x[c + 3]), c2, nref);
-                        y = make_float2(ex2(y.x), ex2(y.y));
-                        z = make_float2(ex2(z.x), ex2(z.y));
-                        s0 = add2(s0, y);
-                        s1 = add2(s1, z);
-                        x[c] = y.x, x[c + 1] = y.y, x[c + 2] = z.x, x[c + 3] = z.y;
-                    }
-                    s0 = add2(s0, s1);
-                    l += s0.x + s0.y;
-                    // pieces by truncation: each takes the next 8 bits, exactly
-                    auto rest = [&]() {
-#pragma unroll
-                        for (int c = 0; c < 64; c += 2) {
-                            const float2 d = add2(make_float2(x[c], x[c + 1]), make_float2(-hi_f(__float_as_uint(x[c])), -hi_f(__float_as_uint(x[c + 1]))));
-                            x[c] = d.x, x[c + 1] = d.y;
-                        }
-                    };
-                    for (int k = 0; SPLIT > 1 && k < warp; ++k) rest();
-#pragma unroll
-                    for (int pc = 0; pc < NP; ++pc) {
-                        if (pc) rest();
+                        l += sum.x + sum.y;
+                        all_of<32 * SPLIT>(true);
                         uint32_t b[32];
 #pragma unroll
-                        for (int c = 0; c < 32; ++c)
-                            b[c] = __byte_perm(__float_as_uint(x[2 * c]), __float_as_uint(x[2 * c + 1]), 0x7632);
-                        ptx::tmem_st32(t_s + 32 * pc, b);
+                        for (int q = 0; q < 8; ++q) {
+                            const uint4 u = *(const uint4*)(xch + warp * 4096 + lane * 128 + ((q ^ (lane & 7)) << 4));
+                            b[4 * q] = u.x, b[4 * q + 1] = u.y, b[4 * q + 2] = u.z, b[4 * q + 3] = u.w;
+                        }
+                        ptx::tmem_st32(t_s, b);
+                    } else {
+                        float x[64];
+                        ptx::tmem_ld64_sync(t_s, x);
+                        if (edge) {
+                            const uint32_t v0 = (uint32_t)vis, v1 = (uint32_t)(vis >> 32);
+#pragma unroll
+                            for (int c = 0; c < 32; ++c) {
+                                if (!(v0 >> c & 1)) x[c] = -INFINITY;
+                                if (!(v1 >> c & 1)) x[32 + c] = -INFINITY;
+                            }
+                        }
+                        float t0 = max3(x[0], x[1], x[2]), t1 = max3(x[3], x[4], x[5]);
+                        float t2 = max3(x[6], x[7], x[8]), t3 = max3(x[9], x[10], x[11]);
+#pragma unroll
+                        for (int c = 12; c < 60; c += 8) {
+                            t0 = max3(t0, x[c], x[c + 1]);
+                            t1 = max3(t1, x[c + 2], x[c + 3]);
+                            t2 = max3(t2, x[c + 4], x[c + 5]);
+                            t3 = max3(t3, x[c + 6], x[c + 7]);
+                        }
+                        t0 = max3(t0, x[60], x[61]);
+                        t1 = max3(t1, x[62], x[63]);
+                        t0 = max3(t0, t1, t2);
+                        const float ref = move(fmaxf(t0, t3) * a.c2);
+                        const float2 nref = make_float2(-ref, -ref);
+                        float2 s0 = make_float2(0.f, 0.f), s1 = s0;
+#pragma unroll
+                        for (int c = 0; c < 64; c += 4) {
+                            float2 y = fma2(make_float2(x[c], x[c + 1]), c2, nref);
+                            float2 z = fma2(make_float2(x[c + 2], x[c + 3]), c2, nref);
+                            y = make_float2(ex2(y.x), ex2(y.y));
+                            z = make_float2(ex2(z.x), ex2(z.y));
+                            s0 = add2(s0, y);
+                            s1 = add2(s1, z);
+                            x[c] = y.x, x[c + 1] = y.y, x[c + 2] = z.x, x[c + 3] = z.y;
+                        }
+                        s0 = add2(s0, s1);
+                        l += s0.x + s0.y;
+#pragma unroll
+                        for (int pc = 0; pc < NP; ++pc) {
+                            uint32_t b[32];
+#pragma unroll
+                            for (int c = 0; c < 32; ++c) {
+                                if (pc) {
+                                    const float2 d = rest(x[2 * c], x[2 * c + 1]);
+                                    x[2 * c] = d.x, x[2 * c + 1] = d.y;
+                                }
+                                b[c] = piece(x[2 * c], x[2 * c + 1]);
+                            }
+                            ptx::tmem_st32(t_s + 32 * pc, b);
+                        }
                     }
                     ptx::tmem_wait_st();
                 }
@@ -728,13 +831,19 @@ __global__ void __launch_bounds__(Cfg<T, KV>::THREADS, Cfg<T, KV>::CTAS)
             odd = !all_of<128>(!odd);
             if (active) {
                 if (odd && (SPLIT == 1 || warp == 0)) add_odd<T, KV>(a, w, g, mine, m == -INFINITY ? 0.f : m, t_lane + COL_O);
+                if constexpr (SPLIT > 1) {  // the windows' sums
+                    ctl.tops[warp * 32 + lane] = l;
+                    all_of<32 * SPLIT>(true);
+                    l = ctl.tops[lane] + (ctl.tops[32 + lane] + ctl.tops[64 + lane]);
+                }
                 const bool whole = w.whole();
                 const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);  // 0: nothing seen
                 const size_t part = (((size_t)worker * a.lanes + tile) * 2 + w.slot()) * ROWS + r;
                 T* out = (T*)a.out + (size_t)(w.q.lo + node) * a.out_ld + (size_t)head * HEAD;
                 auto store = [&](int c, const float (&o)[32]) {
                     if (!mine) return;
-                    if (whole) store_row32<T>(out + c, o, inv);
+                    if (a.parts > 1) store_part(part_o, r, c, o);
+                    else if (whole) store_row32<T>(out + c, o, inv);
                     else store_row32<float>(a.ws_o + part * HEAD + c, o, 1.f);
                 };
                 if constexpr (SPLIT > 1) {  // 64 dims at a time: warp p adds the parts of dims 32 p ..
@@ -768,7 +877,8 @@ __global__ void __launch_bounds__(Cfg<T, KV>::THREADS, Cfg<T, KV>::CTAS)
                     }
                 }
                 if (mine && (SPLIT == 1 || warp == 0)) {
-                    if (!whole) *(float2*)(a.ws_ml + part * 2) = make_float2(m, l);
+                    if (a.parts > 1) part_ml[r] = make_float2(m, l);
+                    else if (!whole) *(float2*)(a.ws_ml + part * 2) = make_float2(m, l);
                     else if (a.lse) a.lse[(size_t)(w.q.lo + node) * a.q_heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
                 }
             }
@@ -779,6 +889,12 @@ __global__ void __launch_bounds__(Cfg<T, KV>::THREADS, Cfg<T, KV>::CTAS)
     }
     __syncwarp();
     __syncthreads();
+    if (a.parts > 1) {
+        ptx::cluster_sync();
+        add_parts<T, C::THREADS>(a, w, rank, row0, shared_rows, ptx::smem_u32(part_o), ptx::smem_u32(part_ml));
+        __syncwarp();
+        ptx::cluster_sync();  // no CTA leaves while its parts are read
+    }
     if (tid == 0 && (ctl.stop || (ptx::smem_u32(sm) & 1023))) flag(a.status, ST_TIMEOUT);
     ptx::tc_fence_after();
     if (warp == W_MMA) ptx::tmem_dealloc(tmem, TMEM_COLS);
@@ -787,22 +903,39 @@ __global__ void __launch_bounds__(Cfg<T, KV>::THREADS, Cfg<T, KV>::CTAS)
 template <typename T, typename KV>
 jl_status launch(const Args& a, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& q, cudaStream_t st) {
     using C = Cfg<T, KV>;
-    return launch_pdl(k_tree_attn_tc<T, KV>, dim3(a.workers, a.lanes), dim3(C::THREADS), tc_smem<C>(), st, a, k, v, q);
+    return launch_pdl_cluster(k_tree_attn_tc<T, KV>, a.parts, dim3(a.workers * a.parts, a.lanes), dim3(C::THREADS), tc_smem<C>(), st, a, k, v, q);
 }
 
 template <typename T, typename KV>
-jl_status configure() {
-    JL_CUDA(cudaFuncSetAttribute(k_tree_attn_tc<T, KV>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tc_smem<Cfg<T, KV>>()));
+jl_status configure(TcLimits& limits) {
+    using C = Cfg<T, KV>;
+    auto kernel = k_tree_attn_tc<T, KV>;
+    JL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tc_smem<C>()));
+    // The call counts one CTA an SM: n of two an SM take the place of n / 2.
+    for (int i = 0; i < TcLimits::SIZES; ++i) {
+        const int n = (2 << i) / C::CTAS;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(n);
+        cfg.blockDim = dim3(C::THREADS);
+        cfg.dynamicSmemBytes = tc_smem<C>();
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = n;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        JL_CUDA(cudaOccupancyMaxActiveClusters(&limits.clusters[C::ROWS_F32][C::POOL_F32][i], kernel, &cfg));
+    }
     return JL_OK;
 }
 
 }  // namespace
 
-jl_status tc_configure() {
-    JL_TRY((configure<float, uint16_t>()));
-    JL_TRY((configure<uint16_t, uint16_t>()));
-    JL_TRY((configure<float, float>()));
-    return configure<uint16_t, float>();
+jl_status tc_configure(TcLimits& limits) {
+    JL_TRY((configure<float, uint16_t>(limits)));
+    JL_TRY((configure<uint16_t, uint16_t>(limits)));
+    JL_TRY((configure<float, float>(limits)));
+    return configure<uint16_t, float>(limits);
 }
 
 jl_status tc_launch(Args a, bool rows_f32, bool pool_f32, cudaStream_t st) {

@@ -185,6 +185,39 @@ def test_long_context(dtype, pool):
 
 
 @types
+@pytest.mark.parametrize("table_pad", [0, 20, 100, 5000])
+@pytest.mark.parametrize("seqs", [1, 3, 24])
+def test_widths_of_the_page_table(dtype, pool, seqs, table_pad):
+    """The work is cut by the pages a sequence may have: whole items, items
+    shared by clusters of CTAs, even ranges.  Sequences without nodes, shorter
+    than a cluster has CTAs, and trees past a tile's rows, in each."""
+    ctx = [(977 * i + 700) % 1500 if i % 5 != 3 else i % 2 for i in range(seqs)]
+    nodes = [(7 * i + 40) % 61 if i % 7 else 33 for i in range(seqs)]
+    Call(make_trees(ctx, nodes, 8, 2, dtype, pool, seed=seqs + table_pad, table_pad=table_pad)).checked()
+
+
+@types
+@pytest.mark.parametrize("table_pad", [8, 100, 5000])
+def test_values_that_are_not_finite_in_shared_items(dtype, pool, table_pad):
+    """Nodes of a tree that spans the parts of an item: a value that only its own
+    row sees reaches no other row."""
+    n = 90
+    t = make_trees([600], [n], 4, 2, dtype, pool, bits=[1 << i for i in range(n)], seed=3, table_pad=table_pad)
+    page, row = t.table[0, 620 // PAGE].item(), 620 % PAGE
+    t.v[page, :, row, 77] = math.inf
+    c = Call(t)
+    c.run()
+    out = c.out[:n, :4 * HEAD].view(n, 4, HEAD)
+    others = torch.arange(n) != 20
+    assert (out[20, :, 77] == math.inf).all()
+    assert torch.isfinite(out[others]).all()
+    t.v[page, :, row, 77] = 0
+    check = Call(t)
+    check.run()
+    assert torch.equal(check.out[:n][others], c.out[:n][others])
+
+
+@types
 def test_captured_and_replayed(dtype, pool):
     """Two calls in one graph, with lengths changed between replays."""
     a = Call(make_trees([300, 20], [7, 30], 4, 2, dtype, pool, seed=16))
