@@ -378,9 +378,10 @@ jl_status jl_qk_norm_rope(const jl_norm_rope* a, void* stream);
  * not reach its output; a value that is not finite in a position that it sees
  * makes that dim of its output infinite or NaN, whatever the position's
  * weight.  Rows from row_start[seqs] on are not written.
- * The sum is split between CTAs by the lengths of the whole batch, in a
- * fixed order: the same inputs give the same bits, but a row's last bits may
- * differ in another batch. */
+ * The sum is split between CTAs by the width of the page table and the
+ * lengths of the whole batch, in a fixed order: the same inputs give the same
+ * bits, but a row's last bits may differ in another batch or with another
+ * max_pages.  A table no wider than the batch needs is fastest. */
 typedef struct jl_tree_attn {
     jl_kv_pages pool;          /* one layer */
     int rows, q_heads;         /* q_heads a multiple of pool.kv_heads, at most 128 per kv head */
