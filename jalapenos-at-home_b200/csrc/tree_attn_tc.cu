@@ -649,7 +649,13 @@ __global__ void __launch_bounds__(Cfg<T, KV>::THREADS, Cfg<T, KV>::CTAS)
                 const bool there = (unsigned)page < (unsigned)a.pages;
                 const bool edge = !there || (p + 1) * PAGE > w.q.ctx;
                 if (i + 1 < n) page = pt[p + 1];
+                ok = ok && wait_phase(&ctl.sfull[it & 1], (it >> 1) & 1, stop);
+                // V only now: these threads do not wait for every page's V, and a phase
+                // is told from the one before the last by the order of the waits alone.
+                // The scores of page `it` are issued after page it - NV's V was waited
+                // for, so the slot's phase cannot be two behind here.
                 if (!C::POOL_F32 && edge && ok) {
+                    static_assert(C::POOL_F32 || NV == 2, "scores are two pages ahead of the products at most");
                     ok = wait_phase(&ctl.vfull[it % NV], (it / NV) & 1, stop);
                     if (ok) {
                         odd |= clean_v(vring + (it % NV) * PAGE_BYTES, max(0, w.q.ctx - p * PAGE),
@@ -657,7 +663,6 @@ __global__ void __launch_bounds__(Cfg<T, KV>::THREADS, Cfg<T, KV>::CTAS)
                         ptx::fence_proxy_async_smem();
                     }
                 }
-                ok = ok && wait_phase(&ctl.sfull[it & 1], (it >> 1) & 1, stop);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok && !(SPLIT > 1 && active)) break;
                 ptx::tc_fence_after();
