@@ -7,7 +7,9 @@
 //   * The softmax thread reads its row's 64 scores, masks those it does not
 //     see (only on pages past the committed positions), and writes the weights
 //     2^(s c2 - m) back over the scores as bf16 pieces, the A operand of the
-//     next MMA: two for bf16 outputs, which leaves 2^-16.
+//     next MMA: two for bf16 outputs, each rounded to nearest, which leaves 2^-17
+//     of a weight at most and no bias (cut off they left up to 2^-15, always low,
+//     and twice as many outputs rounded to the wrong neighbour, in the same time).
 //   * O += P V accumulates in TMEM over the whole segment.  m is the maximum
 //     when it was last moved: it moves, and O is rescaled, only when a row's
 //     maximum has grown by more than 2^8, so that pages seldom touch O.
@@ -695,7 +697,7 @@ __global__ void __launch_bounds__(Cfg<T, KV>::THREADS, Cfg<T, KV>::CTAS)
                         return m == -INFINITY ? 0.f : m;
                     };
                     const uint64_t vis = !edge ? ~0ull : mine && there ? visible(a, w.q, node, p, m0) : 0;
-                    // pieces by truncation: each takes the next 8 bits, exactly
+                    // three pieces by truncation: each takes the next 8 bits, exactly
                     auto piece = [](float x, float y) { return __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632); };
                     auto rest = [](float x, float y) {
                         return add2(make_float2(x, y), make_float2(-hi_f(__float_as_uint(x)), -hi_f(__float_as_uint(y))));
@@ -809,11 +811,11 @@ __global__ void __launch_bounds__(Cfg<T, KV>::THREADS, Cfg<T, KV>::CTAS)
                             uint32_t b[32];
 #pragma unroll
                             for (int c = 0; c < 32; ++c) {
-                                if (pc) {
-                                    const float2 d = rest(x[2 * c], x[2 * c + 1]);
+                                b[c] = pack_bf16(x[2 * c], x[2 * c + 1]);
+                                if (pc + 1 < NP) {
+                                    const float2 d = add2(make_float2(x[2 * c], x[2 * c + 1]), make_float2(-lo_f(b[c]), -hi_f(b[c])));
                                     x[2 * c] = d.x, x[2 * c + 1] = d.y;
                                 }
-                                b[c] = piece(x[2 * c], x[2 * c + 1]);
                             }
                             ptx::tmem_st32(t_s + 32 * pc, b);
                         }

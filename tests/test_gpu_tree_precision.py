@@ -1,0 +1,74 @@
+"""How many bits tree attention keeps: inputs for which every lost bit of a
+weight, a value or a sum adds up in one direction."""
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import jalapeno as J
+from tree_util import Call, HEAD, PAGE, make_trees
+
+pytestmark = pytest.mark.gpu
+
+POOLS = pytest.mark.parametrize("pool", [J.KV_BF16, J.KV_F32], ids=["bf16pool", "f32pool"])
+
+
+def pieces(x, n):
+    """x as n bf16 pieces and their sum in 64 bits."""
+    out, rest = [], x.double()
+    for _ in range(n):
+        out.append(rest.to(torch.bfloat16))
+        rest = rest - out[-1].double()
+    return out, sum(p.double() for p in out)
+
+
+def one_page(pool, nodes, heads, seed):
+    """A sequence of one full page, which all rows see, and nothing else: no row
+    sees a node.  scale 1."""
+    return make_trees([PAGE], [nodes], heads, 1, J.KV_BF16, pool, bits=[0] * nodes, seed=seed, scale=1.0, device="cpu")
+
+
+def to_gpu(t):
+    for f in ("q", "k", "v", "table"):
+        setattr(t, f, getattr(t, f).cuda())
+    return t
+
+
+# What is left in f32, relative to the sum of weighted magnitudes: the
+# exponential (2^-22) and its argument (|s| < 8 and c2 once each, 16 * 2^-24), the sum of
+# 64 weights in 16 steps and their join (18 * 2^-24), at most 16 additions to the
+# accumulator that cut (16 * 2^-23), and the division.
+F32 = 2.0 ** -22 + (16 + 18 + 32 + 2) * 2.0 ** -24
+
+
+def held(out, ref, amp, bits):
+    """Rounded once from within `bits` + F32 of the weighted magnitudes."""
+    half = 2.0 ** (torch.floor(torch.log2(ref.abs())) - 8)
+    far = (out.double() - ref).abs() - half * (1 + 1e-9) - (bits + F32) * amp
+    assert (far <= 0).all(), f"{(far > 0).sum().item()} of {far.numel()} outputs too far, by {far.max().item():.3g}"
+
+
+@POOLS
+def test_weights_are_rounded_to_nearest(pool):
+    """63 keys with one and the same weight, so that what is lost of it is not
+    averaged away, beside one of weight 1 whose value is zero.  Two rounded bf16
+    pieces are 2^-17 of a weight off at most."""
+    nodes, heads = 64, 8
+    t = one_page(pool, nodes, heads, 1)
+    g = torch.Generator().manual_seed(2)
+    a, score = pieces(0.05 + 4 * torch.rand(nodes * heads, generator=g), 3)
+    q = torch.zeros(nodes * heads, HEAD)
+    for d, p in enumerate(a):
+        q[:, d] = p.float()
+    t.q = q.view(nodes, heads * HEAD).to(torch.bfloat16)
+    page = t.table[0, 0].long()
+    t.k[page] = 0
+    t.k[page, :, 1:, :3] = -1
+    v = (1 + torch.rand(HEAD, generator=g)).to(torch.bfloat16)
+    t.v[page] = v.to(t.v.dtype)
+    t.v[page, :, 0] = 0
+    w = torch.exp(-score)
+    ref = (63 * w / (1 + 63 * w))[:, None] * v.double()
+    c = Call(to_gpu(t))
+    c.run()
+    held(c.out.cpu().view(nodes * heads, HEAD), ref, ref, 2.0 ** -17)
