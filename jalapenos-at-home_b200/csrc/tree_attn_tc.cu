@@ -33,8 +33,9 @@
 // Pools of f32 pages: eight warps take the place of the TMA warp.  They load a
 // head's K or V rows into registers, two items ahead, and write them to the rings
 // as bf16 pieces, which S and O then sum: three (24 bits, exact), but two of V for
-// bf16 rows (2^-16 of a value at most, far below the output's rounding).  One CTA
-// fills an SM.  Clearing V happens on the way.
+// bf16 rows, the second rounded (2^-16 of a value at most, far below the output's
+// rounding).  Every piece of a weight meets every piece of V: the product of the
+// two second pieces alone may reach 2^-15.  One CTA fills an SM.  Clearing V happens on the way.
 //
 // B200, times with the joining kernel, pools of bf16: 32 sequences of 64 nodes,
 // 32 heads over 8, at 4096 positions 227 us (610 TFLOP/s of the attention's own
@@ -221,7 +222,6 @@ __device__ __forceinline__ void issue_pv(uint32_t tmem_p, uint32_t v, uint32_t t
     for (int vp = C::VP - 1; vp >= 0; --vp)
 #pragma unroll
         for (int p = C::NP - 1; p >= 0; --p) {
-            if (vp && p) continue;  // both second pieces: below what two pieces leave
 #pragma unroll
             for (int s = 0; s < 4; ++s) {  // keys 16 s ..
                 ptx::mma_bf16_ta(tmem_o, tmem_p + 32 * p + 8 * s, desc(v + ((vp * PAGE_BYTES + 2048 * s) >> 4)), idesc, first ? 0u : 1u);
@@ -351,15 +351,19 @@ struct Items {
     }
 };
 
-// One float4 of a row as n <= N pieces by truncation, each the next 8 bits.  (The
-// last piece rounded: 552 -> 716 us for 4 sequences of 60 nodes, 64 f32 heads over
-// 8, at 2000 positions; the conversions hold the loaders up.)
+// One float4 of a row as n <= N pieces, each the next 8 bits by truncation; three
+// hold all 24.  The second of two is rounded by adding half of what it drops: an
+// addition more costs nothing that was measured (141 us with and without for 8
+// sequences of 24 nodes, 32 bf16 heads over 8, at 4096 positions; conversions that
+// round held the loaders up, 552 -> 716 us for 4 sequences of 60 nodes, 64 f32 heads
+// over 8, at 2000).
 template <int N>
 __device__ __forceinline__ void store_pieces(uint8_t* dst, float4 x, int n) {
 #pragma unroll
     for (int p = 0; p < N; ++p) {
         if (p >= n) break;
-        const uint32_t u0 = __float_as_uint(x.x), u1 = __float_as_uint(x.y), u2 = __float_as_uint(x.z), u3 = __float_as_uint(x.w);
+        const uint32_t up = p == 1 && n == 2 ? 0x8000u : 0u;  // half of what the last of two drops
+        const uint32_t u0 = __float_as_uint(x.x) + up, u1 = __float_as_uint(x.y) + up, u2 = __float_as_uint(x.z) + up, u3 = __float_as_uint(x.w) + up;
         *(uint2*)(dst + p * PAGE_BYTES) = make_uint2(__byte_perm(u0, u1, 0x7632), __byte_perm(u2, u3, 0x7632));
         x = make_float4(x.x - hi_f(u0), x.y - hi_f(u1), x.z - hi_f(u2), x.w - hi_f(u3));
     }

@@ -72,3 +72,49 @@ def test_weights_are_rounded_to_nearest(pool):
     c = Call(to_gpu(t))
     c.run()
     held(c.out.cpu().view(nodes * heads, HEAD), ref, ref, 2.0 ** -17)
+
+
+def test_values_of_an_f32_pool():
+    """bf16 rows, weights of one: values whose low bits are all ones.  Two bf16
+    pieces, the second rounded, are 2^-16 of a value off at most."""
+    nodes, heads = 1, 64
+    t = one_page(J.KV_F32, nodes, heads, 3)
+    g = torch.Generator().manual_seed(4)
+    t.q[:] = 0
+    out = []
+    for _ in range(40):
+        bits = torch.randint(0, 2 ** 7, (HEAD,), generator=g) << 16 | 1 << 15 | torch.randint(0, 2 ** 7, (HEAD,), generator=g) << 8 | 255
+        v = (bits + (127 << 23)).int().view(torch.float32)  # in [1, 2)
+        page = t.table[0, 0].long()
+        t.v[page] = v
+        c = Call(to_gpu(t))
+        c.run()
+        out.append((c.out.cpu().view(nodes * heads, HEAD)[:1], v.double()))
+        t.v = t.v.cpu()
+    held(torch.cat([o for o, _ in out]), torch.stack([v for _, v in out]), torch.stack([v for _, v in out]), 2.0 ** -16)
+
+
+def test_second_pieces_meet():
+    """bf16 rows over an f32 pool: weights and values with second pieces as large
+    as they get."""
+    nodes, heads = 64, 8
+    t = one_page(J.KV_F32, nodes, heads, 5)
+    g = torch.Generator().manual_seed(6)
+    # weights near 0.5 + 2^-9 - 2^-13 and the like: half a step of the first piece above it
+    first = 0.5 + torch.randint(0, 120, (nodes * heads,), generator=g) * 2.0 ** -8
+    a, score = pieces(-torch.log(first.double() + 2.0 ** -9 - 2.0 ** -13), 3)
+    q = torch.zeros(nodes * heads, HEAD)
+    for d, p in enumerate(a):
+        q[:, d] = p.float()
+    t.q = q.view(nodes, heads * HEAD).to(torch.bfloat16)
+    page = t.table[0, 0].long()
+    t.k[page] = 0
+    t.k[page, :, 1:, :3] = -1
+    v = 1 + torch.randint(0, 2 ** 7, (HEAD,), generator=g) * 2.0 ** -7 + 2.0 ** -7 - 2.0 ** -14  # two pieces hold it
+    t.v[page] = v.float()
+    t.v[page, :, 0] = 0
+    w = torch.exp(-score)
+    ref = (63 * w / (1 + 63 * w))[:, None] * v.double()
+    c = Call(to_gpu(t))
+    c.run()
+    held(c.out.cpu().view(nodes * heads, HEAD), ref, ref, 2.0 ** -17)
