@@ -178,6 +178,7 @@ jl_status limits_of(int device, TcLimits& out) {
 // `parts` CTAs, or even ranges of units.
 struct Plan {
     int tile_rows, lanes, workers, min_units, whole, parts;
+    int slots;  // of ws_o for each CTA: 2 partial results, 1 for sums over runs of pages, 0 none
     size_t bytes;
 };
 
@@ -214,10 +215,16 @@ Plan plan_of(const jl_tree_attn& a, int sms, const TcLimits& limits) {
         p.parts = n;
         p.whole = 1;
     }
-    if (a.seqs == 0 || a.max_pages == 0) p.whole = 0, p.parts = 1;  // the workspace of any call is asked for
+    const bool any = a.seqs == 0 || a.max_pages == 0;  // the workspace of any call is asked for
+    if (any) p.whole = 0, p.parts = 1;
     if (p.parts > 1) p.workers = a.seqs * a.pool.kv_heads;
     p.min_units = p.whole ? 1 : 1 + SEG;
-    p.bytes = p.workers == 1 || p.whole ? 0 : (size_t)p.workers * (sizeof(int4) + (size_t)p.lanes * 2 * p.tile_rows * (HEAD + 2) * sizeof(float));
+    const size_t tile = (size_t)p.tile_rows * sizeof(float);
+    p.slots = p.workers > 1 && !p.whole ? 2 : (a.max_pages + p.parts - 1) / p.parts > tc_run(rows_f32, pool_f32) ? 1 : 0;
+    p.bytes = p.slots == 2   ? (size_t)p.workers * (sizeof(int4) + p.lanes * 2 * tile * (HEAD + 2))
+              : p.slots == 1 ? (size_t)p.workers * p.parts * p.lanes * tile * HEAD
+                             : 0;
+    if (any) p.bytes = std::max(p.bytes, (size_t)std::max(p.workers * p.lanes, tc_ctas(pool_f32) * sms) * tile * HEAD);
     return p;
 }
 
@@ -289,13 +296,14 @@ jl_status tree_attention(const jl_tree_attn& a, cudaStream_t st) {
     k.min_units = p.min_units;
     k.whole = p.whole;
     k.parts = p.parts;
+    k.slots = std::max(p.slots, 1);
     k.ws_join = (int4*)a.workspace;
-    k.ws_o = (float*)(k.ws_join + p.workers);
+    k.ws_o = (float*)(k.ws_join + (p.slots == 2 ? p.workers : 0));
     k.ws_ml = k.ws_o + (size_t)p.workers * p.lanes * 2 * p.tile_rows * HEAD;
     k.status = a.status;
     const bool f = a.dtype == JL_KV_F32;
     JL_TRY(tc_launch(k, f, a.pool.dtype == JL_KV_F32, st));
-    if (p.bytes) {
+    if (p.slots == 2) {
         // all blocks resident, at most one per row there may be
         const long long most = (long long)(p.workers - 1) * a.max_nodes * k.group;
         const dim3 grid((unsigned)std::min<long long>((long long)CB_PER_SM * on.sms, most));

@@ -11,7 +11,9 @@
 // (unnormalised output, maximum and sum of every row) in the workspace, and
 // k_tree_combine adds an item's partials in page order.  A worker has at most
 // two partials: the item its range starts in (slot 0) and the item its range
-// ends in (slot 1).  The first worker w whose pages start inside an item says
+// ends in (slot 1).  Until such a result is there, its place holds the sum over
+// the runs of pages so far (tc_run); without partials a CTA has one place for
+// that.  The first worker w whose pages start inside an item says
 // in ws_join[w] what there is to add: the partial of worker w - 1 (slot 1) and
 // those of w, w + 1 .. (slot 0).
 // Where no sequence can have many pages (`whole`), an item is one unit: none is
@@ -55,9 +57,10 @@ struct Args {
     const void* v;
     float c2;          // scale * log2(e)
     int4* ws_join;     // [worker]
-    float* ws_o;       // [worker][lane][slot][tile_rows][HEAD]
+    float* ws_o;       // [CTA along x][lane][slot][tile_rows][HEAD]
     float* ws_ml;      // [worker][lane][slot][tile_rows][2]: maximum (scores times c2), sum
     int workers, lanes, tile_rows, min_units;
+    int slots;         // 2: partial results; 1: only runs (tc_run) are added in ws_o
     int whole;         // items are not split over workers
     int parts;         // CTAs of a cluster that share a worker's only item; 1: none
     int q_tma;         // the tensor-core kernel's queries come by TMA
@@ -291,6 +294,11 @@ __device__ __forceinline__ void finish_row(const Args& a, int lo, int h, int g, 
 // the launch, by the types of the rows (q and out) and of the pool.
 constexpr int tc_tile_rows(bool rows_f32) { return rows_f32 ? 32 : 128; }
 constexpr int tc_ctas(bool pool_f32) { return pool_f32 ? 1 : 2; }
+// Pages of a run: what is added in TMEM before it is added to ws_o.  The tensor
+// core's additions cut off, always towards zero, 2^-25 to 2^-24 of the sum for each
+// on average, and there are 4 a page for every product of pieces: 64 (72 with a
+// rest) and 72 in a run of f32 rows; 512 (576) of bf16 rows, whose rounding is 2^-9.
+constexpr int tc_run(bool rows_f32, bool pool_f32) { return rows_f32 ? (pool_f32 ? 6 : 16) : (pool_f32 ? 32 : 64); }
 struct TcLimits {
     static constexpr int SIZES = 3;
     int clusters[2][2][SIZES];  // of 2, 4, 8 CTAs that run at once, by [rows f32][pool f32]

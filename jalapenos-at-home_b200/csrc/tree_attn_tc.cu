@@ -10,8 +10,12 @@
 //     next MMA: two for bf16 outputs, each rounded to nearest, which leaves 2^-17
 //     of a weight at most and no bias (cut off they left up to 2^-15, always low,
 //     and twice as many outputs rounded to the wrong neighbour, in the same time).
-//   * O += P V accumulates in TMEM over the whole segment.  m is the maximum
-//     when it was last moved: it moves, and O is rescaled, only when a row's
+//   * O += P V accumulates in TMEM over a run of pages (tc_run) and is then added
+//     in the workspace: the tensor core's additions cut off, so over a whole long
+//     segment O came out too small, by 4.7e-5 for f32 rows at 12000 positions and
+//     values of one sign, 1.3e-4 over an f32 pool; by 2.3e-6 and 3.9e-6 in runs.  A
+//     run's end costs 2 to 3 us (24 sequences of 4 f32 nodes at 8000 positions 174 ->
+//     186 us, f32 pool 638 -> 710).  m is the maximum when it was last moved: it moves, and O is rescaled, only when a row's
 //     maximum has grown by more than 2^8, so that pages seldom touch O.
 //   * The scores of page j + 1 are computed while page j's weights are (two S
 //     buffers).
@@ -85,6 +89,7 @@ struct Cfg {
     static constexpr int XCH = SPLIT > 1 ? SPLIT * ROWS * 64 * 4 : 0;  // the exchange: 64 floats of every row and part
     static constexpr int LOADERS = POOL_F32 ? 8 : 1, THREADS = 32 * (5 + LOADERS), CTAS = tc_ctas(POOL_F32);
     static constexpr uint32_t KSLOT = KP * PAGE_BYTES, VSLOT = VP * PAGE_BYTES;
+    static constexpr int RUN = tc_run(ROWS_F32, POOL_F32), REST = RUN / 8;
 };
 constexpr int SB = 2;   // S buffers
 constexpr int WIN = 24;  // keys of a warp that exchanges
@@ -261,6 +266,98 @@ __device__ __forceinline__ bool clean_v(uint8_t* v, int tree_row, int used, int 
     return odd;
 }
 
+// A barrier of the first N softmax threads that tells whether `ok` holds for all.
+template <int N>
+__device__ __forceinline__ bool all_of(bool ok) {
+    uint32_t r;
+    asm volatile(
+        "{\n .reg .pred p, q;\n"
+        " setp.ne.u32 p, %1, 0;\n"
+        " barrier.cta.red.and.pred q, %2, %3, p;\n"
+        " selp.u32 %0, 1, 0, q;\n}"
+        : "=r"(r)
+        : "r"((uint32_t)ok), "n"(N / 32), "n"(N)
+        : "memory");
+    return r != 0;
+}
+
+// Whether a run ends before page i > 0 of a segment's n; a rest of an eighth of a
+// run at most stays with the last.
+template <typename C>
+__device__ __forceinline__ bool run_ends(int i, int n) { return i % C::RUN == 0 && n - i > C::REST; }
+
+// A run's end (tc_run): O is added to acc, in order of the runs, which first gets
+// the factor f for what the rows' maxima have moved since (`add`: it is not the
+// first).  acc: the tile's rows of HEAD floats, in the workspace.
+template <typename C>
+__device__ __noinline__ void save_run(float* acc, uint8_t* xch, uint32_t t_o, int warp, int lane, int live, float f, bool add) {
+    float o[32];
+    if constexpr (C::SPLIT == 1) {
+        acc += (size_t)(32 * warp + lane) * HEAD;
+#pragma unroll 1
+        for (int c = 0; c < HEAD; c += 32) {
+            __syncwarp();
+            ptx::tmem_ld32_sync(t_o + c, o);
+            if (32 * warp + lane >= live) continue;
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+                const float4 v = add ? *(const float4*)(acc + c + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+                *(float4*)(acc + c + e) = make_float4(fmaf(v.x, f, o[e]), fmaf(v.y, f, o[e + 1]), fmaf(v.z, f, o[e + 2]), fmaf(v.w, f, o[e + 3]));
+            }
+        }
+    } else {  // the three parts of 64 dims at a time; then a half warp adds a row
+        constexpr int STEPS = (C::ROWS / 2 + C::SPLIT - 1) / C::SPLIT;
+        const int first = 2 * warp + (lane >> 4), rows = min(live, C::ROWS);
+#pragma unroll 1
+        for (int c = 0; c < HEAD; c += 64) {
+            float4* at = (float4*)(acc + (size_t)first * HEAD + c) + (lane & 15);
+            float4 v[STEPS];
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k)
+                v[k] = add && first + 2 * C::SPLIT * k < rows ? at[2 * C::SPLIT * k * (HEAD / 4)] : make_float4(0.f, 0.f, 0.f, 0.f);
+            __syncwarp();
+#pragma unroll 1
+            for (int d = 0; d < 64; d += 32) {
+                ptx::tmem_ld32_sync(t_o + c + d, o);
+#pragma unroll
+                for (int e = 0; e < 32; e += 4) *xch_at(xch, warp, lane, d + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            }
+            all_of<32 * C::SPLIT>(true);
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k) {
+                const int r = first + 2 * C::SPLIT * k;
+                const float g = __shfl_sync(0xffffffffu, f, r & 31);
+                if (r < rows) {
+                    const float4 u = xch_sum(xch, r, 4 * (lane & 15));
+                    at[2 * C::SPLIT * k * (HEAD / 4)] = make_float4(fmaf(v[k].x, g, u.x), fmaf(v[k].y, g, u.y), fmaf(v[k].z, g, u.z), fmaf(v[k].w, g, u.w));
+                }
+            }
+            __syncwarp();
+            all_of<32 * C::SPLIT>(true);
+        }
+    }
+}
+
+// The last run's end: O gets f times acc added, in the rows of the one warp of a
+// row's that calls this.
+__device__ __noinline__ void load_runs(const float* acc, uint32_t t_o, bool mine, float f) {
+#pragma unroll 1
+    for (int c = 0; c < HEAD; c += 32) {
+        float o[32];
+        uint32_t bits[32];
+        ptx::tmem_ld32_sync(t_o + c, o);
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+            const float4 v = mine ? *(const float4*)(acc + c + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+            bits[e] = __float_as_uint(fmaf(v.x, f, o[e])), bits[e + 1] = __float_as_uint(fmaf(v.y, f, o[e + 1]));
+            bits[e + 2] = __float_as_uint(fmaf(v.z, f, o[e + 2])), bits[e + 3] = __float_as_uint(fmaf(v.w, f, o[e + 3]));
+        }
+        __syncwarp();
+        ptx::tmem_st32(t_o + c, bits);
+    }
+    ptx::tmem_wait_st();
+}
+
 // Adds what clean_v took out to a warp's rows of O: for every node of this
 // segment's pages that a row sees, its weight times the values that are not
 // finite.  Arguments by value: nothing of the caller's moves to the stack.
@@ -367,21 +464,6 @@ __device__ __forceinline__ void store_pieces(uint8_t* dst, float4 x, int n) {
         *(uint2*)(dst + p * PAGE_BYTES) = make_uint2(__byte_perm(u0, u1, 0x7632), __byte_perm(u2, u3, 0x7632));
         x = make_float4(x.x - hi_f(u0), x.y - hi_f(u1), x.z - hi_f(u2), x.w - hi_f(u3));
     }
-}
-
-// A barrier of the first N softmax threads that tells whether `ok` holds for all.
-template <int N>
-__device__ __forceinline__ bool all_of(bool ok) {
-    uint32_t r;
-    asm volatile(
-        "{\n .reg .pred p, q;\n"
-        " setp.ne.u32 p, %1, 0;\n"
-        " barrier.cta.red.and.pred q, %2, %3, p;\n"
-        " selp.u32 %0, 1, 0, q;\n}"
-        : "=r"(r)
-        : "r"((uint32_t)ok), "n"(N / 32), "n"(N)
-        : "memory");
-    return r != 0;
 }
 
 template <typename T>
@@ -587,7 +669,7 @@ __global__ void __launch_bounds__(Cfg<T, KV>::THREADS, Cfg<T, KV>::CTAS)
     } else if (work && warp == W_MMA && lane == 0) {
         const uint32_t q = desc_lo(ptx::smem_u32(sm), 16), kr = desc_lo(ptx::smem_u32(kring), 16);
         const uint32_t vr = desc_lo(ptx::smem_u32(vring), BOX_BYTES);
-        uint32_t it = 0, seg = 0;
+        uint32_t it = 0, seg = 0, run = 0;
         bool ok = true;
         // A wait costs a few hundred cycles even when it is over: those that are
         // over early are made while the weights are still being computed.
@@ -609,13 +691,13 @@ __global__ void __launch_bounds__(Cfg<T, KV>::THREADS, Cfg<T, KV>::CTAS)
             for (int i = 0; ok && i < n; ++i, ++it) {
                 if (i + 1 < n) scores(it + 1);
                 ok = ok && wait_phase(&ctl.vfull[it % NV], (it / NV) & 1, stop);
-                // the last segment's O was read
-                if (i == 0 && seg > 0) ok = ok && wait_phase(&ctl.ofree, (seg - 1) & 1, stop);
+                const bool fresh = i == 0 || run_ends<C>(i, n);  // the last run's O was read
+                if (fresh && run++ > 0) ok = ok && wait_phase(&ctl.ofree, run & 1, stop);
                 if (i + 2 < n) k_here = ptx::mbar_try_wait(&ctl.kfull[(it + 2) % NK], ((it + 2) / NK) & 1);
                 ok = ok && wait_phase(&ctl.pfull[it & 1], (it >> 1) & 1, stop);
                 if (!ok) break;
                 ptx::tc_fence_after();
-                issue_pv<C>(tmem + 64 * (it % SB), vr + (it % NV) * (C::VSLOT >> 4), tmem + COL_O, i == 0);
+                issue_pv<C>(tmem + 64 * (it % SB), vr + (it % NV) * (C::VSLOT >> 4), tmem + COL_O, fresh);
                 ptx::tc_commit(&ctl.vempty[it % NV]);
                 ptx::tc_commit(&ctl.odone[it & 1]);
             }
@@ -644,7 +726,13 @@ __global__ void __launch_bounds__(Cfg<T, KV>::THREADS, Cfg<T, KV>::CTAS)
                 if (lane == 0) ptx::mbar_arrive(&ctl.qfull);
             }
             const int32_t* pt = a.page_table + (size_t)w.s * a.max_pages;
-            float m = -INFINITY, l = 0.f;
+            float m = -INFINITY, l = 0.f, m_run = -INFINITY;  // m_run: m at the end of the last run
+            float* acc = a.ws_o + (((size_t)blockIdx.x * a.lanes + tile) * a.slots + (w.slot() & (a.slots - 1))) * (size_t)(ROWS * HEAD);
+            auto runs_factor = [&]() {
+                const float f = ex2(m_run - (m == -INFINITY ? 0.f : m));
+                m_run = m;
+                return f;
+            };
             bool odd = false;  // this thread took a value out
             int page = pt[w.p0];
             const uint64_t m0 = mine ? first_word(a, w.q, node) : 0;
@@ -684,7 +772,7 @@ __global__ void __launch_bounds__(Cfg<T, KV>::THREADS, Cfg<T, KV>::CTAS)
                             m = top;
                             l *= f;
                         }
-                        if (i > 0 && __any_sync(0xffffffffu, mine && f != 1.f)) {
+                        if (i > 0 && !run_ends<C>(i, n) && __any_sync(0xffffffffu, mine && f != 1.f)) {
                             const uint32_t j = it - 1;  // every earlier P V is done
                             ok = __all_sync(0xffffffffu, wait_phase(&ctl.odone[j & 1], (j >> 1) & 1, stop));
                             ptx::tc_fence_after();
@@ -829,6 +917,19 @@ __global__ void __launch_bounds__(Cfg<T, KV>::THREADS, Cfg<T, KV>::CTAS)
                 ptx::tc_fence_before();
                 __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(&ctl.pfull[it & 1]);
+                if (run_ends<C>(i + 1, n)) {
+                    if (active) {
+                        ok = ok && wait_phase(&ctl.odone[it & 1], (it >> 1) & 1, stop);
+                        ok = SPLIT > 1 ? all_of<32 * SPLIT>(ok) : __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        ptx::tc_fence_after();
+                        const float f = runs_factor();
+                        save_run<C>(acc, xch, t_lane + COL_O, warp, lane, live, f, i >= C::RUN);
+                        ptx::tc_fence_before();
+                        __syncwarp();
+                    }
+                    if (lane == 0) ptx::mbar_arrive(&ctl.ofree);
+                }
             }
             if (ok) {
                 const uint32_t j = it - 1;
@@ -842,6 +943,10 @@ __global__ void __launch_bounds__(Cfg<T, KV>::THREADS, Cfg<T, KV>::CTAS)
             odd = !all_of<128>(!odd);
             if (active) {
                 if (odd && (SPLIT == 1 || warp == 0)) add_odd<T, KV>(a, w, g, mine, m == -INFINITY ? 0.f : m, t_lane + COL_O);
+                if (n > C::RUN + C::REST) {
+                    const float f = runs_factor();
+                    if (SPLIT == 1 || warp == 0) load_runs(acc + (size_t)r * HEAD, t_lane + COL_O, mine, f);
+                }
                 if constexpr (SPLIT > 1) {  // the windows' sums
                     ctl.tops[warp * 32 + lane] = l;
                     all_of<32 * SPLIT>(true);
@@ -849,7 +954,7 @@ __global__ void __launch_bounds__(Cfg<T, KV>::THREADS, Cfg<T, KV>::CTAS)
                 }
                 const bool whole = w.whole();
                 const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);  // 0: nothing seen
-                const size_t part = (((size_t)worker * a.lanes + tile) * 2 + w.slot()) * ROWS + r;
+                const size_t part = (((size_t)worker * a.lanes + tile) * 2 + w.slot()) * ROWS + r;  // partial results only
                 T* out = (T*)a.out + (size_t)(w.q.lo + node) * a.out_ld + (size_t)head * HEAD;
                 auto store = [&](int c, const float (&o)[32]) {
                     if (!mine) return;

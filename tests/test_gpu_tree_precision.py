@@ -6,7 +6,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import jalapeno as J
-from tree_util import Call, HEAD, PAGE, make_trees
+from tree_util import Call, HEAD, PAGE, make_trees, tree_reference
 
 pytestmark = pytest.mark.gpu
 
@@ -118,3 +118,36 @@ def test_second_pieces_meet():
     c = Call(to_gpu(t))
     c.run()
     held(c.out.cpu().view(nodes * heads, HEAD), ref, ref, 2.0 ** -17)
+
+
+@pytest.mark.parametrize("dtype", [J.KV_F32, J.KV_BF16], ids=["f32", "bf16"])
+@POOLS
+def test_long_sums(dtype, pool):
+    """40 sequences of 12000 positions with values of one sign, so that what the
+    additions lose does not cancel.  f32: a run has fewer than 96 additions that cut
+    half of 2^-23 of the running sum on average, which is half of its last value
+    on average, 96 * 2^-25; runs, weights and parts are added to nearest, 250
+    roundings that average out, 16 * 2^-24; and a score's 24 cuts, 24 * 2^-24 of a
+    sum whose largest part is below 8, in weights that sum to one.  bf16: the
+    rounding, and 512 cuts and the pieces (2^-17 and 2^-16)."""
+    seqs, pages, kv_heads = 40, 12, 8
+    t = make_trees([700], [1], kv_heads, kv_heads, dtype, pool, seed=7, spare=0)
+    assert t.k.shape[0] == pages - 1
+    t.v.copy_(1 + t.v.float().abs())
+    width = -(-12001 // PAGE)
+    g = torch.Generator().manual_seed(8)
+    t.table = torch.randint(0, t.k.shape[0], (seqs, width), generator=g).int().cuda()  # pages are shared
+    t.ctx, t.nodes, t.bits = [12000 - 31 * s for s in range(seqs)], [1] * seqs, None
+    t.q = (1.5 * torch.randn((seqs, kv_heads * HEAD), generator=g)).to(t.q.dtype).cuda()
+    c = Call(t)
+    c.run()
+    ref = tree_reference(t)[0]
+    got = c.out.double().view_as(ref)
+    off = ((got - ref).norm(dim=(1, 2)) / ref.norm(dim=(1, 2))).max().item()
+    if dtype == J.KV_F32:
+        assert off < 96 * 2.0 ** -25 + (16 + 24) * 2.0 ** -24, off
+    else:
+        rounded = ((ref.to(c.out.dtype).double() - ref).norm(dim=(1, 2)) / ref.norm(dim=(1, 2))).max().item()
+        bias = ((got - ref).sum() / ref.sum()).abs().item()  # the rounding itself has none
+        assert off < 1.02 * rounded and bias < 512 * 2.0 ** -25 + 2.0 ** -17 + 2.0 ** -16, (off, rounded, bias)
+    assert c.status.item() == 0
