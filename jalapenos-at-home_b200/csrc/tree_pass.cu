@@ -223,20 +223,24 @@ jl_status predict_tree(jl_model* m, jl_cache* c, const uint32_t* ids, const int3
     }
     sl->page_table[0] = c->d_pages;
     cudaStream_t st = m->stream;
-    JL_CUDA(cudaMemcpyAsync(m->pass.hdr, sl->hdr, (1 + chunks) * sizeof(PassHdr), cudaMemcpyHostToDevice, st));
-    JL_CUDA(cudaMemcpyAsync(m->pass.row, sl->row, n * sizeof(RowDesc), cudaMemcpyHostToDevice, st));
-    JL_CUDA(cudaMemcpyAsync(m->pass.head_row, sl->head_row, n * sizeof(int32_t), cudaMemcpyHostToDevice, st));
-    JL_CUDA(cudaMemcpyAsync(m->pass.page_table, sl->page_table, sizeof(int32_t*), cudaMemcpyHostToDevice, st));
-    JL_CUDA(cudaMemcpyAsync(t->dev, t->host, sizeof(TreeBuffers::Desc), cudaMemcpyHostToDevice, st));
-    JL_TRY(stage_end(m, sl, st));
-    const jl_status rs = record_tree_pass(m, c, *t, (int)n);
-    if (rs == JL_OK) {
+    auto queue = [&]() -> jl_status {
+        JL_CUDA(cudaMemcpyAsync(m->pass.hdr, sl->hdr, (1 + chunks) * sizeof(PassHdr), cudaMemcpyHostToDevice, st));
+        JL_CUDA(cudaMemcpyAsync(m->pass.row, sl->row, n * sizeof(RowDesc), cudaMemcpyHostToDevice, st));
+        JL_CUDA(cudaMemcpyAsync(m->pass.head_row, sl->head_row, n * sizeof(int32_t), cudaMemcpyHostToDevice, st));
+        JL_CUDA(cudaMemcpyAsync(m->pass.page_table, sl->page_table, sizeof(int32_t*), cudaMemcpyHostToDevice, st));
+        JL_CUDA(cudaMemcpyAsync(t->dev, t->host, sizeof(TreeBuffers::Desc), cudaMemcpyHostToDevice, st));
+        JL_TRY(stage_end(m, sl, st));
+        JL_TRY(record_tree_pass(m, c, *t, (int)n));
         JL_CUDA(cudaMemcpyAsync(m->host_out, m->pass.out_ids, n * sizeof(uint32_t), cudaMemcpyDeviceToHost, st));
         if (out_logits)
             JL_CUDA(cudaMemcpyAsync(out_logits, m->s.logits, n * m->vocab * sizeof(float), cudaMemcpyDeviceToHost, st));
-    }
-    JL_CUDA(cudaStreamSynchronize(st));
+        return JL_OK;
+    };
+    // Also after an error: what was queued reads t->host and writes the caller's logits.
+    const jl_status rs = queue();
+    const cudaError_t done = cudaStreamSynchronize(st);
     JL_TRY(rs);
+    JL_CUDA(done);
     JL_TRY(check_device_flag(m));
     memcpy(out_ids, m->host_out, n * sizeof(uint32_t));
     c->tree.assign(parents, parents + n);
