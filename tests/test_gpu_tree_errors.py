@@ -22,18 +22,23 @@ static size_t copy_bytes;
 void fake_event(int in) { event_in = in; syncs_after = -1; }
 void fake_copy(int in, size_t bytes) { copy_in = in, copy_bytes = bytes; syncs_after = -1; }
 int fake_syncs(void) { return syncs_after; }  /* since the call that failed; -1: none failed */
+static void* real(const char* name) {  /* the runtime that the engine's library brought along */
+    static void* lib;
+    if (!lib) lib = dlopen("libcudart.so.12", RTLD_LAZY | RTLD_NOLOAD);
+    return dlsym(lib, name);
+}
 
 int cudaEventRecord(void* e, void* s) {
     if (event_in && !--event_in) { syncs_after = 0; return 999; }
-    return ((int (*)(void*, void*))dlsym(RTLD_NEXT, "cudaEventRecord"))(e, s);
+    return ((int (*)(void*, void*))real("cudaEventRecord"))(e, s);
 }
 int cudaMemcpyAsync(void* d, const void* s, size_t n, int kind, void* st) {
     if (copy_in && (!copy_bytes || copy_bytes == n) && !--copy_in) { syncs_after = 0; return 999; }
-    return ((int (*)(void*, const void*, size_t, int, void*))dlsym(RTLD_NEXT, "cudaMemcpyAsync"))(d, s, n, kind, st);
+    return ((int (*)(void*, const void*, size_t, int, void*))real("cudaMemcpyAsync"))(d, s, n, kind, st);
 }
 int cudaStreamSynchronize(void* s) {
     if (syncs_after >= 0) ++syncs_after;
-    return ((int (*)(void*))dlsym(RTLD_NEXT, "cudaStreamSynchronize"))(s);
+    return ((int (*)(void*))real("cudaStreamSynchronize"))(s);
 }
 """
 
