@@ -328,18 +328,19 @@ jl_status page_unshare(jl_cache* c, size_t i, size_t rows, cudaStream_t stream) 
     jl_model* m = c->m;
     int32_t src = c->pages[i], dst = 0;
     JL_TRY(page_take(m, &dst));
-    if (rows) {
+    auto queue = [&]() -> jl_status {
         const int32_t r = (int32_t)rows;
-        const jl_status s = kv_copy_pages(pages_of(m, 0, m->layers), &src, &dst, &r, 1, stream);
-        if (s != JL_OK) {
-            page_release(m, dst);
-            return s;
-        }
-    }
-    c->pages[i] = c->h_pages[i] = dst;
-    page_release(m, src);
-    JL_CUDA(cudaMemcpyAsync(c->d_pages + i, c->h_pages + i, sizeof(int32_t), cudaMemcpyHostToDevice, stream));
-    return JL_OK;
+        if (rows) JL_TRY(kv_copy_pages(pages_of(m, 0, m->layers), &src, &dst, &r, 1, stream));
+        c->h_pages[i] = dst;
+        JL_CUDA(cudaMemcpyAsync(c->d_pages + i, c->h_pages + i, sizeof(int32_t), cudaMemcpyHostToDevice, stream));
+        return JL_OK;
+    };
+    const jl_status rs = queue();
+    // After an error the device's table still names the shared page, and so must the cache.
+    if (rs != JL_OK) c->h_pages[i] = src;
+    c->pages[i] = c->h_pages[i];
+    page_release(m, rs == JL_OK ? src : dst);
+    return rs;
 }
 
 }  // namespace jl

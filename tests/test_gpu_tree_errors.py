@@ -93,3 +93,31 @@ for arm in (lambda: fake.fake_event(1), lambda: fake.fake_copy(1, 5 * cfg.vocab 
     assert ids == want and np.array_equal(lg, wlg)
 print("ok")
 """)
+
+
+def test_a_failed_unsharing_leaves_the_fork_alone(tmp_path):
+    """The copy of a new page's table entry: after the error the cache still
+    holds the shared page, and its next write copies it first."""
+    child(tmp_path, """
+prompt = O.prompt_ids(128, cfg.vocab, 5)
+a, c = m.cache(), m.cache()
+m.predict(prompt, a)
+m.predict(prompt, c)
+f = a.fork()
+a.truncate(70)
+fake.fake_copy(1, 4)
+try:
+    m.predict(O.prompt_ids(40, cfg.vocab, 8), a)
+    raise SystemExit("no error")
+except J.JlError as e:
+    assert e.status == J.JL_ERR_CUDA, e
+assert a.len == 70
+m.predict(O.prompt_ids(40, cfg.vocab, 8), a)
+for t in (1, 2):
+    assert np.array_equal(m.predict([t], f, logits=True)[1], m.predict([t], c, logits=True)[1])
+g = m.cache()
+m.predict(prompt[:70], g)
+m.predict(O.prompt_ids(40, cfg.vocab, 8), g)
+assert np.array_equal(m.predict([9], a, logits=True)[1], m.predict([9], g, logits=True)[1])
+print("ok")
+""")
