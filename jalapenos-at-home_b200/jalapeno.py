@@ -226,6 +226,18 @@ def u32(a) -> np.ndarray:
     return np.ascontiguousarray(np.asarray(a, dtype=np.int64).astype(np.uint32))
 
 
+def _whole(a, dtype, what: str) -> np.ndarray:
+    """A sequence of whole numbers as `dtype`; ValueError where one does not fit
+    (ctypes and numpy would wrap it to another node or page)."""
+    x = np.asarray(a)
+    if x.size == 0:
+        x = x.astype(np.int64)
+    lim = np.iinfo(dtype)
+    if x.dtype.kind not in "iu" or (x.size and (int(x.min()) < lim.min or int(x.max()) > lim.max)):
+        raise ValueError(f"{what} must be whole numbers in {lim.min}..{lim.max}")
+    return np.ascontiguousarray(x.astype(dtype))
+
+
 def _p(a: np.ndarray, ctype):
     return a.ctypes.data_as(ctypes.POINTER(ctype))
 
@@ -371,7 +383,7 @@ class Model:
         returns the next token after each node's path (jl_predict_tree).
         ``cache.compact(path)`` then keeps a path of the nodes."""
         t = u32(tokens)
-        p = np.ascontiguousarray(np.asarray(parents, dtype=np.int32))
+        p = _whole(parents, np.int32, "parents")
         if p.shape != t.shape:
             raise ValueError("one parent for each token")
         out = np.zeros(max(len(t), 1), np.uint32)
@@ -526,7 +538,7 @@ class Cache:
     def compact(self, path) -> None:
         """Keeps a path of the nodes of the last ``predict_tree``
         (jl_cache_compact)."""
-        p = u32(path)
+        p = _whole(path, np.uint32, "path")
         check(lib.jl_cache_compact(self._h, _p(p, ctypes.c_uint32), len(p)))
 
 
@@ -758,8 +770,8 @@ def kv_copy_pages(pool: KvPages, src, dst, rows=None, stream: int = 0) -> None:
     n = len(src)
     if len(dst) != n or (rows is not None and len(rows) != n):
         raise ValueError("src, dst and rows must have the same length")
-    ints = ctypes.c_int32 * n
-    check(lib.jl_kv_copy_pages(pool, ints(*src), ints(*dst), None if rows is None else ints(*rows), n, stream))
+    lists = [None if x is None else _whole(x, np.int32, "src, dst and rows") for x in (src, dst, rows)]
+    check(lib.jl_kv_copy_pages(pool, *(None if x is None else _p(x, ctypes.c_int32) for x in lists), n, stream))
 
 
 def _philox4x32_10(c0, c1, c2, c3, k0: int, k1: int):
