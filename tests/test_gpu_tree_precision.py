@@ -120,6 +120,53 @@ def test_second_pieces_meet():
     held(c.out.cpu().view(nodes * heads, HEAD), ref, ref, 2.0 ** -17)
 
 
+def tails_of_24_bits(pool, rows, seed):
+    """Queries, keys, values and weights whose third pieces matter: a row's q and
+    the keys' k are one number each with 24 random bits, so that a score is one
+    product, the weight of 63 keys its exponential, and the output that weight
+    times a value, beside one key of weight 1 and value 0.  Returns (a, kappa, v):
+    score -a * kappa; over a bf16 pool kappa is 1 and v is bf16."""
+    g = torch.Generator().manual_seed(seed)
+    a = (0.05 + 7 * torch.rand(rows, generator=g)).float()
+    v = 1 + torch.rand(HEAD, generator=g)
+    if pool == J.KV_BF16:
+        return a, 1.0, v.to(torch.bfloat16).float()
+    return a, float(torch.tensor(1 + 2.0 ** -7 - 2.0 ** -14 - 2.0 ** -16 + 2.0 ** -17, dtype=torch.float32)), v
+
+
+# A score is below 8; its pieces' products are exact, and of the additions the
+# cuts of the first part (two, 2^-23 each) and the two roundings of the parts' sum
+# count, 6 half steps of 2^-24, of 8 taken; the weight is off by that relatively.
+# The output's own rounding is f32's.
+KEPT = F32 + 8 * 8 * 2.0 ** -24 + 2.0 ** -24
+
+
+def far_of(out, a, kappa, v):
+    w = torch.exp(-a.double() * kappa)
+    ref = (63 * w / (1 + 63 * w))[:, None] * v.double()
+    return ((out.double() - ref).abs() / ref).amax().item()
+
+
+@POOLS
+def test_f32_rows_keep_24_bits(pool):
+    """Every third piece, of Q, of the weights and of an f32 pool's K and V: without
+    one of them the largest error is several times the bound (next test)."""
+    nodes, heads = 64, 8
+    t = one_page(pool, nodes, heads, 9)
+    a, kappa, v = tails_of_24_bits(pool, nodes * heads, 10)
+    q = torch.zeros(nodes * heads, HEAD)
+    q[:, 5] = a
+    t.q = q.view(nodes, heads * HEAD)
+    page = t.table[0, 0].long()
+    t.k[page] = 0
+    t.k[page, :, 1:, 5] = -kappa
+    t.v[page] = v.to(t.v.dtype)
+    t.v[page, :, 0] = 0
+    c = Call(to_gpu(t))
+    c.run()
+    assert far_of(c.out.cpu().view(nodes * heads, HEAD), a, kappa, v) <= KEPT
+
+
 @pytest.mark.parametrize("dtype", [J.KV_F32, J.KV_BF16], ids=["f32", "bf16"])
 @POOLS
 def test_long_sums(dtype, pool):
