@@ -187,7 +187,9 @@ jl_status jl_predict_draft(jl_model* m, jl_cache* c, const uint32_t* ids, size_t
  * out_ids[i] is the model's next token after the committed positions and node
  * i's path.  A chain (parents -1, 0, 1, ..) predicts what jl_predict with `all`
  * set does, up to the rounding of other kernels (logits within 2e-4 relative L2
- * on a bf16 pool).  1..JL_TREE_MAX_NODES nodes, at most max_pass_rows, and
+ * on a bf16 pool): where a row's two best logits are nearer than that, the two
+ * calls may name different tokens, and decoding by trees may leave the stream
+ * that jl_generate or jl_generate_speculative gives.  1..JL_TREE_MAX_NODES nodes, at most max_pass_rows, and
  * length + n within the context limit.  The length stays; jl_cache_compact
  * keeps a path.  The reference verifies chains only (speculative.rs:95-97).
  * out_logits (nullable) receives [n, vocab] f32 logits. */
@@ -371,8 +373,15 @@ jl_status jl_qk_norm_rope(const jl_norm_rope* a, void* stream);
  * node's own bit included: nothing is added to the mask).  Without a mask
  * the nodes form a chain: node i sees nodes 0..i, as in a prompt, a decode
  * step or a linear verify pass.
- *   out = sum over seen p of softmax(q . k_p * scale) v_p, in f32, rounded
- *   once into the output type; lse = log of the sum of exp(q . k_p * scale).
+ *   out = sum over seen p of softmax(q . k_p * scale) v_p, rounded once into
+ *   the output type; lse = log of the sum of exp(q . k_p * scale).
+ * Scores, maxima and sums are f32; q . k_p * scale must stay below 2^30.  The
+ * exponential is off by 2^-22 of itself, and weights below 2^-126 of the row's
+ * largest are zero.  f32 rows: q, k, v and the weights keep 24 bits.  bf16 rows:
+ * the weights keep 17 bits and an f32 pool's values 16, both rounded to nearest.
+ * The tensor core's additions cut off, so long sums are carried on in f32 outside
+ * it: what is lost stays below 6e-6 of the weighted mean of |v| for f32 rows, and
+ * below 4e-5 before the rounding for bf16 rows, whatever the length.
  * A row that sees nothing gets zeros and an lse of -infinity.  Whatever lies
  * in positions that a row does not see, infinities and NaN included, does
  * not reach its output; a value that is not finite in a position that it sees
@@ -392,7 +401,8 @@ typedef struct jl_tree_attn {
     size_t out_ld;             /* a multiple of 8 */
     float* lse;                /* [rows][q_heads], or NULL */
     int seqs;
-    int max_nodes;             /* largest tree of the batch, 1..JL_TREE_MAX_NODES */
+    int max_nodes;             /* largest tree of the batch, 1..JL_TREE_MAX_NODES; CTAs are set
+                                  aside for its rows in every sequence, so no larger than needed */
     const int32_t* row_start;  /* [seqs + 1] */
     const int32_t* ctx;        /* [seqs] */
     const uint64_t* mask;      /* [rows][mask_words]: bit j % 64 of word j / 64, or NULL */
@@ -421,7 +431,7 @@ typedef struct jl_kv_compaction {
     const int32_t* path;       /* [seqs][path_ld] node indices */
     int path_ld;               /* 1..JL_TREE_MAX_NODES */
     const int32_t* path_len;   /* [seqs], each at most path_ld */
-    const int32_t* page_table; /* [seqs][max_pages]; no page written by two sequences */
+    const int32_t* page_table; /* [seqs][max_pages]; a page that one sequence writes to is no other's */
     int max_pages;
     int32_t* status;
 } jl_kv_compaction;

@@ -33,7 +33,7 @@ template <typename T>
 __global__ void __launch_bounds__(CB_T, CB_PER_SM) k_tree_combine(Args a) {
     __shared__ float4 share_o[CB_WARPS][32];
     __shared__ float2 share_ml[CB_WARPS];
-    __shared__ int before[CB_MOST + 1];  // groups of CB_WARPS rows before item i
+    __shared__ int before[CB_MOST + 1];  // groups of rows (CB_ROWS or one) before item i
     __shared__ short who[CB_MOST];       // item i is ws_join[who[i]], kept in joins[i]
     __shared__ int4 joins[CB_MOST];
     __shared__ int2 warp_sums[CB_WARPS];

@@ -41,14 +41,17 @@
 // rounding).  Every piece of a weight meets every piece of V: the product of the
 // two second pieces alone may reach 2^-15.  One CTA fills an SM.  Clearing V happens on the way.
 //
-// B200, times with the joining kernel, pools of bf16: 32 sequences of 64 nodes,
-// 32 heads over 8, at 4096 positions 227 us (610 TFLOP/s of the attention's own
-// products, 914 with the second piece); one of 16 nodes at 40000 positions 44 us,
-// 37 of one node at 4096 positions 110 us (5.6 TB/s, 86% of the copy rate).
-// Small trees over long contexts are bound by the pages' bytes (1.45 us a page
-// and CTA is the copy rate), large ones by the MMAs, whose issuing thread is held
-// up by the pipe two thirds of the time; short ones by the chain of lookups,
-// copies and first instructions (about 6 us) and by the joining kernel (5 us).
+// B200, GPU times of calls in a graph with the joining kernel, bf16 rows and
+// pools, 32 heads over 8: 32 sequences of 64 nodes at 4096 positions 240 us in a
+// burst of 20 calls (580 TFLOP/s of the attention's own products, 860 with the
+// second piece) and 282 us in a loop of seconds, where the power cap takes the
+// clock from 1.9 to 1.55 GHz; one of 16 nodes at 40000 positions 46 to 52 us; 37 of
+// one node at 4096 positions 118 us (5.3 TB/s, 80% of the copy rate).  Small trees
+// over long contexts are bound by the pages' bytes (1.45 us a page and CTA is the
+// copy rate); large ones by the chain of a page, with two CTAs an SM to overlap it
+// (tensor pipe 48% of active cycles, exponentials 33%; 8 sequences of 64 nodes at
+// 8192 positions); short ones by the chain of lookups, copies and first
+// instructions (about 6 us) and by the joining kernel (5 us).
 // Tried and not kept: eight softmax warps, two threads a row (272 -> 297 us for
 // the first case: exchanging the maxima costs more than it saves); the scores of
 // two pages as one MMA group of 128 columns (227 -> 252 us: the next scores no
